@@ -88,6 +88,25 @@ class ArGroup(ctypes.Structure):
     ]
 
 
+class AttnDesc(ctypes.Structure):
+    """aib_attn_desc (include/afterimage_b200.h)."""
+    _fields_ = [
+        ("q", P), ("k", P), ("v", P), ("out", P),
+        ("q_batch_stride", I64), ("q_token_stride", I64), ("q_head_stride", I64),
+        ("k_batch_stride", I64), ("k_head_stride", I64), ("k_token_stride", I64),
+        ("v_batch_stride", I64), ("v_head_stride", I64), ("v_token_stride", I64),
+        ("out_batch_stride", I64), ("out_token_stride", I64), ("out_head_stride", I64),
+        ("tokens", I64), ("batch", I64), ("key_rows", I64),
+        ("nh", I32), ("nkv", I32), ("hd", I32),
+        ("scale", ctypes.c_float),
+        ("cu_q", P), ("cu_k", P), ("len_k", P), ("pos", P), ("mask", P),
+        ("mask_batch_stride", I64), ("mask_row_stride", I64), ("mask_col_stride", I64),
+        ("mask_cols", I64),
+        ("workspace", P),
+        ("workspace_floats", I64),
+    ]
+
+
 # (name, restype, argtypes) of every exported entry point; tests check that
 # the header declares exactly these.
 SIGNATURES = [
@@ -131,6 +150,12 @@ SIGNATURES = [
     ("aib_gemv_bf16", CI, [P, I64, P, I64, P, I64, I64, I64, CI, CI, P]),
     ("aib_gemm_bf16_tc", CI, [P, I64, P, I64, P, I64, I64, I64, I64, P, I64, P, P]),
     ("aib_gemm_bf16_tc_workspace_floats", I64, [I64, I64, I64]),
+    ("aib_attention_workspace_floats", I64, [ctypes.POINTER(AttnDesc)]),
+    ("aib_prompt_attention_bf16", CI, [ctypes.POINTER(AttnDesc), P, P]),
+    ("aib_tree_attention_bf16", CI, [ctypes.POINTER(AttnDesc), P, P]),
+    ("aib_rope_cache_packed_bf16", CI, [P, I64, I64, I64, CI, CI, CI, P, P, P, P, P, ctypes.c_float, P, P, P, P, P, P,
+                                        I64, P]),
+    ("aib_keep_cache_rows_bf16", CI, [P, CI, I64, CI, I64, CI, P, P, P, CI, P]),
 ]
 
 

@@ -320,6 +320,74 @@ int aib_gemm_bf16_tc(const void *w, int64_t ldw, const void *x, int64_t ldx, voi
                      void *stream);
 int64_t aib_gemm_bf16_tc_workspace_floats(int64_t m, int64_t n, int64_t k);
 
+/* ------------------------------------------------------------------------
+ * Passes of more than one token over cached sequences: packed prompts and
+ * trees of drafted tokens. They replace the attention and rotary math of
+ * transformers' Qwen3 / Llama modules that the reference runs around its
+ * hooks (afterimage/runtime/streaming_engine.py:1871-1915), one sequence at a
+ * time; its speculation loop (:2488-2575) has no cache. BF16 throughout,
+ * scores, softmax sums and outputs accumulated in fp32 and rounded once.
+ * Strides are in elements, the head size is contiguous. Work on `stream`.
+ * ------------------------------------------------------------------------ */
+typedef struct aib_attn_desc {
+  const void *q;   /* prompt: [tokens, nh, hd]; tree: [batch, tokens, nh, hd] */
+  const void *k;   /* caches: [batch, nkv, key_rows, hd]; packed: [key_rows, nkv, hd] */
+  const void *v;   /* as k */
+  void *out;       /* as q */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t k_batch_stride, k_head_stride, k_token_stride;
+  int64_t v_batch_stride, v_head_stride, v_token_stride;
+  int64_t out_batch_stride, out_token_stride, out_head_stride;
+  int64_t tokens;  /* prompt: query rows of all sequences; tree: queries of each sequence */
+  int64_t batch;   /* sequences */
+  int64_t key_rows;
+  int32_t nh, nkv, hd; /* kv head = head / (nh / nkv); hd <= 256 */
+  float scale;
+  const int64_t *cu_q;  /* prompt: device int64[batch + 1], first query row of each sequence */
+  const int64_t *cu_k;  /* prompt, packed keys: device int64[batch + 1] */
+  const int64_t *len_k; /* prompt, caches: device int64[batch], keys of each sequence (NULL: packed) */
+  const int64_t *pos;   /* tree: device int64[batch], slot of the first drafted token */
+  const uint8_t *mask;  /* tree: [batch, tokens, mask_cols], nonzero where the query sees the drafted column */
+  int64_t mask_batch_stride, mask_row_stride, mask_col_stride;
+  int64_t mask_cols;    /* tree: drafted tokens in the cache, at slots pos .. pos + mask_cols - 1 */
+  float *workspace;     /* aib_attention_workspace_floats(desc) floats (NULL when 0); each call in flight
+                           needs its own */
+  int64_t workspace_floats;
+} aib_attn_desc;
+
+/* Floats of workspace the descriptor's call needs (0: none). The pointers
+ * need not be set except for their being NULL or not. */
+int64_t aib_attention_workspace_floats(const aib_attn_desc *desc);
+/* Causal attention of packed prompts: sequence b has the query rows
+ * cu_q[b] .. cu_q[b + 1] - 1 (m of them) and L keys; its row i sees the keys
+ * j <= L - m + i, so that its queries stand at the end of its keys. Rows
+ * that see nothing are zero; rows outside every sequence are not written.
+ * Offsets are cut to the tensors' extents. d_status (optional): a bounded
+ * wait that gives up sets AIB_STATUS_WAIT_TIMEOUT. */
+int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream);
+/* Attention of drafted tokens over caches: every query of sequence b sees
+ * the slots before pos[b], and slot pos[b] + j where mask[b, i, j]. Slots
+ * outside [0, key_rows) are not seen. */
+int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream);
+/* qkv [n, (nh + 2 nkv) * hd] with row stride qkv_stride; row cu[b] + i is
+ * token i of sequence b. RMSNorm of q and k over hd (when both weights are
+ * given), rotary embedding at place start[b] + depth[row] (depth NULL: i),
+ * q -> q_out [n, nh, hd], k and v -> row start[b] + i of sequence b's caches
+ * ({batch, head, row} strides; rows outside [0, max_len) are not written).
+ * fp32 between the reads and one rounding at the writes. */
+int aib_rope_cache_packed_bf16(const void *qkv, int64_t qkv_stride, int64_t n, int64_t batch, int nh, int nkv, int hd,
+                               const int64_t *cu, const int64_t *start, const int64_t *depth, const void *q_norm_w,
+                               const void *k_norm_w, float eps, const float *inv_freq, void *q_out, void *k_cache,
+                               void *v_cache, const int64_t *k_strides, const int64_t *v_strides, int64_t max_len,
+                               void *stream);
+/* In each of `count` caches (host array of device pointers, all [batch, nkv,
+ * max_len, hd] with the same {batch, head, row} strides): row pos[b] + i <-
+ * row pos[b] + keep[b, i] as it was before the call, for i < n (n <= 256).
+ * keep < 0, and rows outside [0, max_len), leave the row as it is. The
+ * tensors must not overlap. */
+int aib_keep_cache_rows_bf16(void *const *tensors, int count, int64_t batch, int nkv, int64_t max_len, int hd,
+                             const int64_t *strides, const int64_t *pos, const int64_t *keep, int n, void *stream);
+
 /* Elementwise recombine of an already-decoded exponent field: replaces
  * recombine_exponent_and_sign_mantissa / _recombine
  * (afterimage/runtime/compressed_store.py:94-130). */
