@@ -11,11 +11,15 @@
 // cache slot before pos, and slot pos + j where mask[i, j]. A row that sees
 // nothing is zero. What a row does not see cannot reach it: masked scores are
 // replaced, not added to, and a masked v_j is never multiplied.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <mutex>
 
 #include "aib_internal.h"
 
@@ -163,6 +167,802 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
 }
 
 // ---------------------------------------------------------------------------
+// The tensor-core kernel (head sizes that are multiples of 8, up to 128).
+//
+// A tile is 128 rows: the G = nh / nkv heads that share a kv head, for
+// 128 / G tokens (row r = token r / G, head r mod G). Sharing heads fills the
+// rows of the matrix instructions for short prompts and drafted trees, and
+// makes one pass over a kv head's keys serve all its queries. A CTA takes two
+// tiles of consecutive tokens over the same keys ("pair"), or one tile whose
+// key tiles two streams take in turn and join at the end ("solo"), and,
+// where that would leave SMs empty, a share of the key axis; the shares are
+// joined by a second kernel.
+//
+// Per CTA, 128 keys at a time:
+//   S = Q K^T         tcgen05.mma, both operands in shared memory -> tensor memory
+//   P = exp2(S - m)   one thread per row: running maximum and sum, P as BF16
+//                     over S's columns in tensor memory
+//   O = O + P V       tcgen05.mma, P from tensor memory, V as it lies in
+//                     shared memory (keys x head size)
+// The running maximum is only followed when it would leave P above 2^8: any
+// reference m gives the same quotient, and rescaling O costs a pass over it.
+//
+// Warps 0-3 and 4-7: the softmax of stream 0 and 1; warp 8: TMA loads into a
+// ring of K and V tiles; warp 9: the matrix instructions; warps 10-11: where
+// a key tile is not seen in full, they replace what is not finite in V by
+// zero, since a masked weight of zero times NaN is NaN; what of it is seen by
+// some row is added back, row by row, at the end.
+// Every wait is bounded; one that gives up sets AIB_STATUS_WAIT_TIMEOUT and
+// the CTA unwinds.
+// ---------------------------------------------------------------------------
+constexpr int kTile = 128;
+constexpr int kThreads = 384;
+constexpr int kMaxSlots = 8;
+constexpr unsigned kWaitLimit = AIB_WAIT_LIMIT_POLLS;
+constexpr float kFollow = 8.f;  // log2 of how far above 1 a weight may come before the maximum is followed
+
+template <int HDP>
+struct Cfg {
+  static constexpr int kHalves = HDP / 64;             // 128-byte-swizzled column blocks of a tile
+  static constexpr int kSlotBytes = kHalves * 16384;   // one K, V or Q tile
+  static constexpr int kSlots = HDP == 128 ? 5 : 8;
+  static constexpr int kSmem = (2 + kSlots) * kSlotBytes + 1024;
+};
+
+struct TcParams {
+  aib_attn_desc d;
+  int group, tt;       // heads per kv head, tokens per tile
+  int tpi;             // tiles an item may hold: 2 or 1
+  int splits;          // shares of the key axis
+  int items;           // upper bound of the items
+  float scale_log2;
+  int vec_out;         // output rows allow 16-byte stores
+  int32_t *status;
+};
+
+// What one CTA works on.
+struct Item {
+  Seq s;
+  int64_t t0;          // first token of tile 0 within the sequence
+  int cnt[2];          // tokens in each tile
+  int64_t end[2];      // keys that some row of the tile sees lie before this
+  int64_t low[2];      // every row of the tile sees the keys before this
+  int ta, tb;          // key tiles of this share
+  bool live;
+};
+
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Item number -> sequence and first tile. Prompts: items are numbered from
+// the last tiles of the longest prompts down (they see the most keys; the
+// hardware hands CTAs out in order, so the longest run first). With P_b items
+// in sequence b, the items at level l (the l-th of their sequence) or above
+// are F(l) = sum_b max(0, P_b - l); a binary search finds the item's level.
+// Collective over the warp.
+__device__ __forceinline__ bool find_item(const TcParams &p, int64_t item, int64_t &b, int64_t &level) {
+  const int64_t unit = static_cast<int64_t>(p.tt) * p.tpi;
+  const int64_t batch = p.d.batch;
+  if (p.d.mask) {
+    const int64_t per = (p.d.tokens + unit - 1) / unit;
+    b = item / per;
+    level = item - b * per;
+    return b < batch;
+  }
+  const int lane = threadIdx.x & 31;
+  const auto items_of = [&](int64_t i) {
+    const int64_t q0 = clamp64(p.d.cu_q[i], 0, p.d.tokens);
+    return (clamp64(p.d.cu_q[i + 1], q0, p.d.tokens) - q0 + unit - 1) / unit;
+  };
+  if (batch == 1) {
+    b = 0;
+    level = items_of(0) - 1 - item;
+    return level >= 0;
+  }
+  const int64_t first = lane < batch ? items_of(lane) : 0;  // the common case needs no second read
+  const auto at_or_above = [&](int64_t l) {
+    int64_t f = first > l ? first - l : 0;
+    for (int64_t i = lane + 32; i < batch; i += 32) {
+      const int64_t n = items_of(i);
+      if (n > l) f += n - l;
+    }
+    return warp_sum(f);
+  };
+  if (at_or_above(0) <= item) return false;
+  int64_t lo = 0, hi = (p.d.tokens + unit - 1) / unit;  // F(lo) > item >= F(hi)
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (at_or_above(mid) > item) lo = mid; else hi = mid;
+  }
+  int64_t rank = item - at_or_above(lo + 1);  // among the sequences that reach this level
+  for (int64_t i0 = 0; i0 < batch; i0 += 32) {
+    const int64_t i = i0 + lane;
+    unsigned has = __ballot_sync(0xffffffffu, i < batch && (i0 == 0 ? first : items_of(i)) > lo);
+    if (rank < __popc(has)) {
+      for (; rank > 0; --rank) has &= has - 1;
+      b = i0 + __ffs(has) - 1;
+      level = lo;
+      return true;
+    }
+    rank -= __popc(has);
+  }
+  return false;
+}
+
+__device__ __forceinline__ Item make_item(const TcParams &p, int64_t item, int split) {
+  Item w;
+  int64_t b = 0, level = 0;
+  w.live = find_item(p, item, b, level);
+  if (!w.live) return w;
+  w.s = sequence(p.d, b);
+  w.t0 = level * p.tt * p.tpi;
+  int64_t most = 0;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int64_t t = w.t0 + static_cast<int64_t>(s) * p.tt;
+    w.cnt[s] = s < p.tpi ? static_cast<int>(clamp64(w.s.m - t, 0, p.tt)) : 0;
+    if (p.d.mask) {
+      w.end[s] = w.s.L;
+      w.low[s] = clamp64(w.s.off, 0, w.s.L);
+    } else {
+      w.end[s] = clamp64(w.s.off + t + w.cnt[s], 0, w.s.L);
+      w.low[s] = clamp64(w.s.off + t + 1, 0, w.s.L);
+    }
+    if (w.cnt[s] == 0) w.end[s] = 0;
+    most = w.end[s] > most ? w.end[s] : most;
+  }
+  const int tiles = static_cast<int>((most + kTile - 1) / kTile);
+  const int per = (tiles + p.splits - 1) / p.splits;
+  w.ta = min(tiles, split * per);
+  w.tb = min(tiles, w.ta + per);
+  return w;
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, unsigned parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// true when the phase of `parity` completed within the bound; gives up early when another role did
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity, volatile int *gave_up) {
+  for (unsigned n = 0; n < kWaitLimit; ++n) {
+    if (mbar_try(bar, parity)) return true;
+    if (n > 256) {
+      if (*gave_up) break;
+      __nanosleep(32);
+    }
+  }
+  *gave_up = 1;
+  return false;
+}
+
+// the same for a whole warp: one answer, so that its lanes stay together
+__device__ __forceinline__ bool warp_wait(uint32_t bar, unsigned parity, volatile int *gave_up) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up));
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
+// shared-memory matrix descriptors, 128-byte swizzle. K-major (Q, K): 128-byte
+// rows, 8-row groups 1024 bytes apart. MN-major (V, rows are keys): 64 columns
+// a block, blocks of 64 columns 16 KiB apart, 8-key groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_base(uint32_t addr, uint64_t lead) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (lead << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) { return desc_base(addr, 1); }
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) { return desc_base(addr, 16384 >> 4); }
+
+// BF16 x BF16 -> F32, M = 128
+__host__ __device__ constexpr uint32_t idesc_bf16(int n, int b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn_major) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | ((kTile >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+#define AIB_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define AIB_I8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+
+// 32 tensor-memory columns of this thread's lane
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : AIB_R8(v, 0), AIB_R8(v, 8), AIB_R8(v, 16), AIB_R8(v, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      AIB_I8(v, 0), AIB_I8(v, 8), AIB_I8(v, 16), AIB_I8(v, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      AIB_I8(v, 0), AIB_I8(v, 8)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two floats as packed BF16, `lo` in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
+
+// bits of the seen keys among the four 32-key words of key tile t, for this
+// thread's row (token tok of the tile; first token of the tile is ti within
+// the sequence). Collective over the warp for trees.
+__device__ __forceinline__ void seen_words(const TcParams &p, const Item &w, int s, int tok, int warp_tok0,
+                                           int warp_tok1, int t, uint32_t (&bits)[4]) {
+  const int64_t key0 = static_cast<int64_t>(t) * kTile;
+  const int64_t i = w.t0 + static_cast<int64_t>(s) * p.tt + tok;
+  if (!p.d.mask) {
+    const int64_t n = clamp64(w.s.off + i + 1, 0, w.s.L) - key0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t k = n - 32 * c;
+      bits[c] = k >= 32 ? 0xffffffffu : (k <= 0 ? 0u : (1u << static_cast<int>(k)) - 1u);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const uint8_t *m = p.d.mask + w.s.qb * p.d.mask_batch_stride;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) bits[c] = 0;
+  for (int a = warp_tok0; a <= warp_tok1; ++a) {
+    const uint8_t *row = m + (w.t0 + static_cast<int64_t>(s) * p.tt + a) * p.d.mask_row_stride;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t key = key0 + 32 * c + lane;
+      const int64_t col = key - w.s.off;
+      bool seen = key < w.s.L && col < p.d.mask_cols;
+      if (seen && col >= 0) seen = row[col * p.d.mask_col_stride] != 0;
+      const uint32_t word = __ballot_sync(0xffffffffu, seen);
+      if (a == tok) bits[c] = word;
+    }
+  }
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
+  using C = Cfg<HDP>;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t bar_full[kMaxSlots], bar_empty[kMaxSlots];
+  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2], bar_o[2], bar_drain, bar_dirty, bar_clean;
+  __shared__ uint32_t tmem_base;
+  __shared__ int gave_up, bad_seen;
+  __shared__ float join[2][kTile];  // maximum and sum of stream 1's rows
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x % p.d.nkv;
+  const int rest = blockIdx.x / p.d.nkv;
+  const int split = rest % p.splits;
+  const Item w = make_item(p, rest / p.splits, split);
+  if (!w.live) return;  // uniform over the CTA: no barrier or tensor memory is held yet
+
+  const bool pair = w.cnt[1] > 0;
+  // pair: key tiles of each stream; solo: the tiles that both take in turn
+  int n[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int e = static_cast<int>((w.end[s] + kTile - 1) / kTile);
+    n[s] = max(0, min(e, w.tb) - w.ta);
+  }
+  const int nk = pair ? max(n[0], n[1]) : n[0];
+  const int my_n[2] = {pair ? n[0] : (nk + 1) / 2, pair ? n[1] : nk / 2};
+  // the first key tile of this share that some row does not see in full
+  const int64_t low = pair ? min(w.low[0], w.low[1]) : w.low[0];
+  const int first_masked = static_cast<int>(max(static_cast<int64_t>(0), low / kTile - w.ta));
+
+  const uint32_t smem_q = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t ring = smem_q + 2 * C::kSlotBytes;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), 1);
+      mbar_init(smem_u32(&bar_empty[i]), 1);
+    }
+    mbar_init(smem_u32(&bar_q), 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&bar_s[s]), 1);
+      mbar_init(smem_u32(&bar_p[s]), 4);
+      mbar_init(smem_u32(&bar_o[s]), 1);
+    }
+    mbar_init(smem_u32(&bar_drain), 1);
+    mbar_init(smem_u32(&bar_dirty), 1);
+    mbar_init(smem_u32(&bar_clean), 2);
+    gave_up = 0;
+    bad_seen = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_base;
+  const uint32_t tmem_s[2] = {tmem, tmem + 128};
+  const uint32_t tmem_o[2] = {tmem + 256, tmem + 384};
+
+  // ring positions of the K and V tiles, in the order in which the matrix instructions want them
+  const auto pos_k = [&](int j) { return pair ? 2 * j : (j == 0 ? 0 : 2 * j - 1); };
+  const auto pos_v = [&](int j) { return pair ? 2 * j + 1 : (j == nk - 1 ? 2 * nk - 1 : 2 * j + 2); };
+
+  if (warp == 8) {
+    if (lane == 0 && nk > 0) {
+      const int kb = static_cast<int>(w.s.kb), qb = static_cast<int>(w.s.qb);
+      const uint32_t qbar = smem_u32(&bar_q);
+      const uint32_t qbytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(qbar),
+                   "r"(pair ? 2 * qbytes : qbytes)
+                   : "memory");
+      for (int s = 0; s < (pair ? 2 : 1); ++s)
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group,
+                      static_cast<int>(w.s.q0 + w.t0) + s * p.tt, qb, qbar);
+      int issued = 0;
+      for (int pos = 0; pos < 2 * nk; ++pos) {
+        const int slot = pos % C::kSlots;
+        const unsigned ph = static_cast<unsigned>(pos / C::kSlots) & 1u;
+        if (!mbar_wait(smem_u32(&bar_empty[slot]), ph ^ 1u, &gave_up)) break;
+        bool is_v;
+        int j;
+        if (pair) {
+          is_v = pos & 1;
+          j = pos >> 1;
+        } else {
+          is_v = pos > 0 && (pos % 2 == 0 || pos == 2 * nk - 1);
+          j = pos == 0 ? 0 : (pos == 2 * nk - 1 ? nk - 1 : (is_v ? pos / 2 - 1 : (pos + 1) / 2));
+        }
+        const uint32_t fb = smem_u32(&bar_full[slot]);
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"(C::kSlotBytes) : "memory");
+        const int row = static_cast<int>(w.s.k0) + (w.ta + j) * kTile;
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, is_v ? &map_v : &map_k, h * 64, row, kvh, kb, fb);
+        issued = pos + 1;
+      }
+      // copies in flight land before the CTA can end (bounded)
+      (void)mbar_wait(qbar, 0, &gave_up);
+      for (int pos = max(0, issued - C::kSlots); pos < issued; ++pos)
+        for (unsigned k = 0; k < kWaitLimit; ++k) {
+          if (mbar_try(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u)) break;
+          __nanosleep(32);
+        }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && nk > 0) {
+      constexpr uint32_t id_s = idesc_bf16(kTile, 0), id_o = idesc_bf16(HDP, 1);
+      unsigned clean_ph = 0, p_ph[2] = {0, 0};
+      bool o_open[2] = {false, false};  // has the stream's O been written?
+      bool ok = mbar_wait(smem_u32(&bar_q), 0, &gave_up);
+      const auto wait_full = [&](int pos) {
+        return mbar_wait(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u, &gave_up);
+      };
+      const auto scores = [&](int s, int pos) {  // S of stream s from the K tile at ring position pos
+        const uint32_t q = smem_q + (pair ? s : 0) * C::kSlotBytes, k = ring + (pos % C::kSlots) * C::kSlotBytes;
+#pragma unroll
+        for (int i = 0; i < C::kHalves * 4; ++i) {
+          const uint32_t o = (i / 4) * 16384 + (i % 4) * 32;
+          mma_ss(tmem_s[s], desc_kmajor(q + o), desc_kmajor(k + o), id_s, i > 0);
+        }
+        mma_commit(smem_u32(&bar_s[s]));
+      };
+      const auto values = [&](int s, int pos) {  // O of stream s from its P and the V tile at pos
+        const uint32_t v = ring + (pos % C::kSlots) * C::kSlotBytes;
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+          mma_ts(tmem_o[s], tmem_s[s] + i * 8, desc_mnmajor(v + i * 2048), id_o, (i > 0 || o_open[s]) ? 1u : 0u);
+        o_open[s] = true;
+      };
+      // V tile j has landed; warps 10-11 look it over (while the softmax runs) where some row does not see all of it
+      const auto wait_v = [&](int j, int pos) {
+        if (!wait_full(pos)) return false;
+        if (j >= first_masked) mbar_arrive(smem_u32(&bar_dirty));
+        return true;
+      };
+      const auto wait_clean = [&](int j) {
+        if (j < first_masked) return true;
+        const bool r = mbar_wait(smem_u32(&bar_clean), clean_ph, &gave_up);
+        clean_ph ^= 1u;
+        return r;
+      };
+      const auto wait_p = [&](int s) {
+        const bool r = mbar_wait(smem_u32(&bar_p[s]), p_ph[s], &gave_up);
+        p_ph[s] ^= 1u;
+        return r;
+      };
+      const auto release = [&](int pos) { mma_commit(smem_u32(&bar_empty[pos % C::kSlots])); };
+      if (ok && pair) {
+        ok = wait_full(0);
+        fence_after();
+        if (ok) {
+          if (n[0] > 0) scores(0, 0);
+          scores(1, 0);
+          release(0);
+        }
+        for (int j = 0; ok && j < nk; ++j) {
+          const int pv = pos_v(j), pk = pos_k(j + 1);
+          if (!(ok = wait_v(j, pv))) break;
+          const bool more = j + 1 < nk;
+          if (j < n[0] && !(ok = wait_p(0))) break;
+          if (!(ok = wait_clean(j))) break;
+          if (j < n[0]) {
+            fence_after();
+            values(0, pv);
+            if (j + 1 == n[0]) mma_commit(smem_u32(&bar_o[0]));
+          }
+          if (more) {
+            if (!(ok = wait_full(pk))) break;
+            fence_after();
+            if (j + 1 < n[0]) scores(0, pk);
+          }
+          if (!(ok = wait_p(1))) break;
+          fence_after();
+          values(1, pv);
+          release(pv);
+          if (more) {
+            scores(1, pk);
+            release(pk);
+          } else {
+            mma_commit(smem_u32(&bar_o[1]));
+          }
+        }
+      } else if (ok) {
+        ok = wait_full(0);
+        fence_after();
+        if (ok) {
+          scores(0, 0);
+          release(0);
+        }
+        for (int j = 0; ok && j < nk; ++j) {
+          const int s = j & 1;
+          if (j + 1 < nk) {
+            const int pk = pos_k(j + 1);
+            if (!(ok = wait_full(pk))) break;
+            fence_after();
+            scores(s ^ 1, pk);
+            release(pk);
+          }
+          const int pv = pos_v(j);
+          if (!(ok = wait_v(j, pv)) || !(ok = wait_p(s)) || !(ok = wait_clean(j))) break;
+          fence_after();
+          values(s, pv);
+          release(pv);
+          if (j + 2 >= nk) mma_commit(smem_u32(&bar_o[s]));
+        }
+      }
+      // nothing of this CTA is in flight in the tensor core when it ends
+      mma_commit(smem_u32(&bar_drain));
+      for (unsigned k = 0; k < kWaitLimit && !mbar_try(smem_u32(&bar_drain), 0); ++k) __nanosleep(32);
+    }
+  } else if (warp >= 10) {
+    // ---- V tiles that some row does not see in full: what is not finite becomes zero
+    const int64_t seen_end = w.end[0] > w.end[1] ? w.end[0] : w.end[1];
+    const int self = static_cast<int>(threadIdx.x) - 320;
+    for (int j = first_masked; j < nk; ++j) {
+      if (!warp_wait(smem_u32(&bar_dirty), (j - first_masked) & 1u, &gave_up)) break;
+      const uint32_t base = ring + (pos_v(j) % C::kSlots) * C::kSlotBytes;
+      const int64_t rows_seen = seen_end - static_cast<int64_t>(w.ta + j) * kTile;
+      for (int e = self; e < C::kSlotBytes / 16; e += 64) {
+        uint32_t x[4];
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                     : "r"(base + e * 16)
+                     : "memory");
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (not_finite_bf16(x[i])) x[i] &= 0xffff0000u, found = true;
+          if (not_finite_bf16(x[i] >> 16)) x[i] &= 0x0000ffffu, found = true;
+        }
+        if (found) {
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + e * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                       "r"(x[3])
+                       : "memory");
+          if ((e % 1024) / 8 < rows_seen) bad_seen = 1;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_clean));
+    }
+  } else {
+    // ---- softmax: one thread per row of the stream's tile
+    const int s = warp >> 2;
+    const int tile = pair ? s : 0;
+    const int wrow = (warp & 3) * 32, row = wrow + lane;
+    const int rows = w.cnt[tile] * p.group;
+    const bool active = wrow < rows;  // a warp without rows only keeps the barriers going
+    const int tok = min(row / p.group, w.cnt[tile] - 1);
+    const int tok0 = wrow / p.group, tok1 = min((wrow + 31) / p.group, w.cnt[tile] - 1);
+    const uint32_t lanes = static_cast<uint32_t>(wrow) << 16;
+    const uint32_t ts = tmem_s[s] + lanes, to = tmem_o[s] + lanes;
+    const float sl = p.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    const int mine = my_n[s];
+    bool ok = true;
+    for (int it = 0; it < mine; ++it) {
+      const int j = pair ? it : 2 * it + s;
+      const int t = w.ta + j;
+      const bool masked = (static_cast<int64_t>(t) + 1) * kTile > w.low[tile];
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      if (masked && active) seen_words(p, w, tile, tok, tok0, tok1, t, bits);
+      if (!(ok = warp_wait(smem_u32(&bar_s[s]), it & 1, &gave_up))) break;
+      fence_after();
+      if (active) {
+        uint32_t x[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, x + 32 * c);
+        tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (!((bits[i / 32] >> (i % 32)) & 1u)) x[i] = 0xff800000u;  // -infinity
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 128; ++i) top[i % 4] = fmaxf(top[i % 4], __uint_as_float(x[i]));
+        const float mz = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
+        const bool follow = mz > m + kFollow;
+        if (__any_sync(0xffffffffu, follow)) {
+          const float mn = follow ? mz : m;
+          const float a = m == -INFINITY ? 0.f : ex2(m - mn);
+          if (it > 0) {
+            // the stream's previous P V is done: its S was ready only after it
+#pragma unroll
+            for (int c = 0; c < HDP / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+              tmem_st32(to + 32 * c, o);
+            }
+          }
+          l *= a;
+          m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = ex2(fmaf(__uint_as_float(x[32 * c + 2 * i]), sl, -ref));
+            const float e1 = ex2(fmaf(__uint_as_float(x[32 * c + 2 * i + 1]), sl, -ref));
+            sum[i % 4] += e0 + e1;
+            pk[i] = pack_bf16(e0, e1);  // the matrix product takes BF16; the sum keeps fp32
+          }
+          tmem_st16(ts + 16 * c, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_p[s]));
+    }
+    if (ok && mine > 0) ok = warp_wait(smem_u32(&bar_o[s]), 0, &gave_up);
+    fence_after();
+
+    // what V held that is not finite and this row sees, in one column block
+    const auto add_bad = [&](float *o, int c0) {
+      const uint16_t *v = static_cast<const uint16_t *>(p.d.v) + w.s.kb * p.d.v_batch_stride +
+                          w.s.k0 * p.d.v_token_stride + kvh * p.d.v_head_stride;
+      for (int it = 0; it < mine; ++it) {
+        const int j = pair ? it : 2 * it + s;
+        if (j < first_masked) continue;
+        uint32_t bits[4];
+        seen_words(p, w, tile, tok, tok0, tok1, w.ta + j, bits);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          for (int i = 0; i < 32; ++i) {
+            const int64_t key = static_cast<int64_t>(w.ta + j) * kTile + 32 * c + i;
+            if (key >= w.s.L || !((bits[c] >> i) & 1u)) continue;
+            const uint16_t *vr = v + key * p.d.v_token_stride;
+#pragma unroll
+            for (int d = 0; d < 32; ++d)
+              if (c0 + d < p.d.hd && not_finite_bf16(vr[c0 + d])) o[d] += b2f(vr[c0 + d]);
+          }
+      }
+    };
+    const bool fix = __any_sync(0xffffffffu, *static_cast<volatile int *>(&bad_seen) != 0);
+    float *joined = reinterpret_cast<float *>(raw + (ring - smem_u32(raw)));  // [HDP][128], over the ring
+
+    if (!pair) {
+      // solo: stream 1's maximum, sum and O go through shared memory; both streams' matrix work is done first
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (s == 1) {
+        join[0][row] = m;
+        join[1][row] = l;
+        if (active && ok && mine > 0)
+#pragma unroll
+          for (int c = 0; c < HDP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * c, o);
+            tmem_wait_ld();
+            if (fix) add_bad(reinterpret_cast<float *>(o), 32 * c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) joined[(32 * c + i) * kTile + row] = __uint_as_float(o[i]);
+          }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if ((pair || s == 0) && active && ok) {
+      float a0 = 1.f, a1 = 0.f;
+      const bool second = !pair && my_n[1] > 0;
+      if (second) {
+        const float m1 = join[0][row], mm = fmaxf(m, m1);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        a0 = ex2(m - ref);
+        a1 = ex2(m1 - ref);
+        l = l * a0 + join[1][row] * a1;
+        m = mm;
+      }
+      const bool valid = row < rows;
+      const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      const int64_t unit = (static_cast<int64_t>(rest) * p.d.nkv + kvh) * p.tpi + tile;
+      float *part = p.d.workspace + unit * (kTile * (HDP + 2));
+      const int64_t token = w.s.q0 + w.t0 + static_cast<int64_t>(tile) * p.tt + tok;
+      uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
+                      (kvh * p.group + row % p.group) * p.d.out_head_stride;
+#pragma unroll
+      for (int c = 0; c < HDP / 32; ++c) {
+        float o[32];
+        if (mine > 0) {
+          tmem_ld32(to + 32 * c, reinterpret_cast<uint32_t *>(o));
+          tmem_wait_ld();
+          if (fix) add_bad(o, 32 * c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (second) o[i] = o[i] * a0 + joined[(32 * c + i) * kTile + row] * a1;
+          o[i] = l == 0.f ? 0.f : o[i] * inv;
+        }
+        if (!valid) continue;
+        if (p.splits > 1) {
+          if (mine == 0) continue;  // the sum of zero written below says that there is nothing
+#pragma unroll
+          for (int i = 0; i < 32; ++i) part[(32 * c + i) * kTile + row] = o[i];
+        } else if (p.vec_out) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (32 * c + i < p.d.hd)
+              *reinterpret_cast<uint4 *>(out + 32 * c + i) =
+                  make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]),
+                             pack_bf16(o[i + 6], o[i + 7]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i < p.d.hd) out[32 * c + i] = f2b(o[i]);
+        }
+      }
+      if (p.splits > 1 && valid) {
+        part[HDP * kTile + row] = m;
+        part[(HDP + 1) * kTile + row] = l;
+      }
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && gave_up && p.status) atomicOr(p.status, AIB_STATUS_WAIT_TIMEOUT);
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// Joins the shares of the key axis: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
+// A block takes 32 rows of one tile, a warp 8 of their columns.
+template <int HDP>
+__global__ void __launch_bounds__(HDP * 4) attn_join_kernel(const __grid_constant__ TcParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t u = blockIdx.x;
+  const int quarter = static_cast<int>(u % 4);
+  u /= 4;
+  const int tile = static_cast<int>(u % p.tpi);
+  u /= p.tpi;
+  const int kvh = static_cast<int>(u % p.d.nkv);
+  const int64_t item = u / p.d.nkv;
+  const Item w = make_item(p, item, 0);
+  if (!w.live) return;
+  const int row = quarter * 32 + lane;
+  if (row >= w.cnt[tile] * p.group) return;
+  const int c0 = warp * 8;
+  if (c0 >= p.d.hd) return;
+  const auto part = [&](int sp) {
+    return p.d.workspace + (((item * p.splits + sp) * p.d.nkv + kvh) * p.tpi + tile) * (kTile * (HDP + 2));
+  };
+  // a share that the item's key tiles do not reach holds nothing: the CTA wrote a sum of zero there
+  float m = -INFINITY;
+  for (int sp = 0; sp < p.splits; ++sp) m = fmaxf(m, part(sp)[HDP * kTile + row]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[8] = {};
+  for (int sp = 0; sp < p.splits; ++sp) {
+    const float *q = part(sp);
+    const float ls = q[(HDP + 1) * kTile + row];
+    if (ls == 0.f) continue;
+    const float a = ex2(q[HDP * kTile + row] - ref);
+    l += a * ls;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] += a * q[(c0 + i) * kTile + row];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] *= inv;
+  const int64_t token = w.s.q0 + w.t0 + static_cast<int64_t>(tile) * p.tt + row / p.group;
+  uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
+                  (kvh * p.group + row % p.group) * p.d.out_head_stride + c0;
+  if (p.vec_out) {
+    *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]),
+                                                 pack_bf16(o[6], o[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c0 + i < p.d.hd) out[i] = f2b(o[i]);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 static int check_common(const aib_attn_desc *p, const char *who) {
@@ -179,11 +979,157 @@ static int check_common(const aib_attn_desc *p, const char *who) {
   return AIB_OK;
 }
 
-static int launch(const aib_attn_desc &p, const char *who, cudaStream_t st) {
-  const int64_t rows = (p.mask ? p.batch : 1) * p.tokens * p.nh;
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_fn() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(p);
+  });
+  return fn;
+}
+
+// 4-D BF16 tensor (innermost first), box 64 columns x box1 x box2, 128-byte swizzle, zero fill outside
+static bool make_map(CUtensorMap *map, const void *base, const int64_t (&size)[4], const int64_t (&stride)[3], int box1,
+                     int box2) {
+  EncodeTiled enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[4], strides[3];
+  for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(size[i]);
+  // the stride of a dimension of one is never used
+  for (int i = 0; i < 3; ++i) strides[i] = size[i + 1] > 1 ? static_cast<cuuint64_t>(stride[i]) * 2 : 16;
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box1), static_cast<cuuint32_t>(box2), 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// a dimension that the TMA can step over: 16-byte steps, forward, no expanded tensor
+static bool tma_stride(int64_t size, int64_t stride) {
+  return size <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1LL << 38));
+}
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The tensor-core kernel takes head sizes that are multiples of 8 up to 128,
+// at most 128 heads per kv head, a positive scale (the maximum of the scores
+// is taken before it) and what the TMA can address; the plain kernel takes
+// the rest.
+static bool tensor_cores(const aib_attn_desc &d, bool tree) {
+  const int64_t b = tree ? d.batch : 1, kb = tree || d.len_k ? d.batch : 1;
+  return d.hd % 8 == 0 && d.hd <= 128 && d.nh / d.nkv <= kTile && d.scale > 0.f && d.key_rows > 0 && aligned16(d.q) &&
+         aligned16(d.k) && aligned16(d.v) && tma_stride(d.tokens, d.q_token_stride) &&
+         tma_stride(d.nh, d.q_head_stride) && tma_stride(b, d.q_batch_stride) &&
+         tma_stride(d.key_rows, d.k_token_stride) && tma_stride(d.nkv, d.k_head_stride) &&
+         tma_stride(kb, d.k_batch_stride) && tma_stride(d.key_rows, d.v_token_stride) &&
+         tma_stride(d.nkv, d.v_head_stride) && tma_stride(kb, d.v_batch_stride);
+}
+
+struct TcPlan {
+  int group, tt, tpi, splits;
+  int64_t items;
+};
+
+static int64_t item_bound(const aib_attn_desc &d, bool tree, int64_t unit) {
+  if (tree) return d.batch * ((d.tokens + unit - 1) / unit);
+  // the sum of ceil(m_b / unit) over sequences whose m_b add up to at most `tokens`
+  return std::min(d.tokens, (d.tokens + d.batch * (unit - 1)) / unit);
+}
+
+static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
+  TcPlan pl;
+  pl.group = d.nh / d.nkv;
+  pl.tt = kTile / pl.group;
+  pl.tpi = 2;
+  pl.splits = 1;
+  pl.items = item_bound(d, tree, 2LL * pl.tt);
+  // two tiles over the same keys halve the loads, but only where that still gives every SM an item
+  if (pl.items * d.nkv < sms) {
+    pl.tpi = 1;
+    pl.items = item_bound(d, tree, pl.tt);
+    const int64_t units = std::max<int64_t>(1, pl.items * d.nkv);
+    // shares of at least two key tiles (one for each stream), at most one CTA per SM
+    const int64_t tiles = (d.key_rows + kTile - 1) / kTile;
+    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, (tiles + 1) / 2)));
+  }
+  return pl;
+}
+
+static int64_t tc_floats(const aib_attn_desc &d, const TcPlan &pl) {
+  if (pl.splits == 1) return 0;
+  const int hdp = d.hd <= 64 ? 64 : 128;
+  return pl.items * pl.splits * d.nkv * pl.tpi * kTile * (hdp + 2);
+}
+
+static int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+template <int HDP>
+static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, int32_t *status,
+                     cudaStream_t st) {
+  // the shared-memory limit is set once per device
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(ready.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HDP>::kSmem);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
+  }
+  if (e != cudaSuccess) return aib_set_errorf("%s: %s", who, cudaGetErrorString(e)), AIB_ECUDA;
+  const int64_t kb = tree || d.len_k ? d.batch : 1;
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, d.q, {d.hd, d.nh, d.tokens, tree ? d.batch : 1},
+                {d.q_head_stride, d.q_token_stride, d.q_batch_stride}, pl.group, pl.tt) ||
+      !make_map(&mk, d.k, {d.hd, d.key_rows, d.nkv, kb}, {d.k_token_stride, d.k_head_stride, d.k_batch_stride}, kTile,
+                1) ||
+      !make_map(&mv, d.v, {d.hd, d.key_rows, d.nkv, kb}, {d.v_token_stride, d.v_head_stride, d.v_batch_stride}, kTile,
+                1))
+    return aib_set_errorf("%s: cuTensorMapEncodeTiled failed", who), AIB_ECUDA;
+  TcParams p;
+  p.d = d;
+  p.group = pl.group;
+  p.tt = pl.tt;
+  p.tpi = pl.tpi;
+  p.splits = pl.splits;
+  p.items = static_cast<int>(pl.items);
+  p.scale_log2 = d.scale * 1.4426950408889634f;
+  p.vec_out = aligned16(d.out) && d.out_token_stride % 8 == 0 && d.out_head_stride % 8 == 0 &&
+              d.out_batch_stride % 8 == 0;
+  p.status = status;
+  const int64_t grid = pl.items * pl.splits * d.nkv;
+  attn_tc_kernel<HDP><<<static_cast<unsigned>(grid), kThreads, Cfg<HDP>::kSmem, st>>>(mq, mk, mv, p);
+  if ((e = cudaGetLastError()) == cudaSuccess && pl.splits > 1) {
+    attn_join_kernel<HDP><<<static_cast<unsigned>(pl.items * d.nkv * pl.tpi * 4), HDP * 4, 0, st>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return aib_set_errorf("%s: %s", who, cudaGetErrorString(e)), AIB_ECUDA;
+  return AIB_OK;
+}
+
+static int launch(const aib_attn_desc &d, const char *who, int32_t *status, cudaStream_t st) {
+  const bool tree = d.mask != nullptr;
+  if (tensor_cores(d, tree)) {
+    const TcPlan pl = tc_plan(d, tree, sm_count());
+    if (pl.items * pl.splits * d.nkv * 4 * pl.tpi > INT32_MAX) return aib_set_errorf("%s: too many rows", who), AIB_EINVAL;
+    const int64_t need = tc_floats(d, pl);
+    if (need && (!d.workspace || d.workspace_floats < need))
+      return aib_set_errorf("%s: needs a workspace of %lld floats", who, (long long)need), AIB_EINVAL;
+    return d.hd <= 64 ? launch_tc<64>(d, tree, pl, who, status, st) : launch_tc<128>(d, tree, pl, who, status, st);
+  }
+  const int64_t rows = (tree ? d.batch : 1) * d.tokens * d.nh;
   const int64_t blocks = (rows + kPlainWarps - 1) / kPlainWarps;
   if (blocks > INT32_MAX) return aib_set_errorf("%s: too many rows", who), AIB_EINVAL;
-  attn_plain_kernel<<<static_cast<unsigned>(blocks), kPlainWarps * 32, 0, st>>>(p);
+  attn_plain_kernel<<<static_cast<unsigned>(blocks), kPlainWarps * 32, 0, st>>>(d);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return aib_set_errorf("%s: %s", who, cudaGetErrorString(e)), AIB_ECUDA;
   return AIB_OK;
@@ -193,7 +1139,7 @@ static int launch(const aib_attn_desc &p, const char *who, cudaStream_t st) {
 
 using namespace aibseq;
 
-AIB_API int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *, void *stream) {
+AIB_API int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream) {
   const char *who = "prompt_attention";
   if (const int rc = check_common(desc, who)) return rc;
   aib_attn_desc p = *desc;
@@ -202,10 +1148,10 @@ AIB_API int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *, void
   if (!p.q || !p.out || !p.cu_q || (p.key_rows && (!p.k || !p.v)))
     return aib_set_errorf("%s: null pointer", who), AIB_EINVAL;
   if (!p.len_k && !p.cu_k) return aib_set_errorf("%s: give cu_k (packed keys) or len_k (caches)", who), AIB_EINVAL;
-  return launch(p, who, static_cast<cudaStream_t>(stream));
+  return launch(p, who, d_status, static_cast<cudaStream_t>(stream));
 }
 
-AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *, void *stream) {
+AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream) {
   const char *who = "tree_attention";
   if (const int rc = check_common(desc, who)) return rc;
   const aib_attn_desc &p = *desc;
@@ -215,7 +1161,11 @@ AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *, void *
   if (p.tokens == 0 || p.batch == 0) return AIB_OK;
   if (!p.q || !p.out || !p.pos || !p.mask || (p.key_rows && (!p.k || !p.v)))
     return aib_set_errorf("%s: null pointer", who), AIB_EINVAL;
-  return launch(p, who, static_cast<cudaStream_t>(stream));
+  return launch(p, who, d_status, static_cast<cudaStream_t>(stream));
 }
 
-AIB_API int64_t aib_attention_workspace_floats(const aib_attn_desc *) { return 0; }
+AIB_API int64_t aib_attention_workspace_floats(const aib_attn_desc *d) {
+  if (check_common(d, "attention_workspace_floats") || d->tokens == 0 || d->batch == 0) return 0;
+  const bool tree = d->mask != nullptr;
+  return tensor_cores(*d, tree) ? tc_floats(*d, tc_plan(*d, tree, sm_count())) : 0;
+}

@@ -51,6 +51,31 @@ def test_packed_prompts(nh, nkv, hd, lens):
     R.check(got, *R.prompt(q, k, v, cu, hd ** -0.5)[:2])
 
 
+@pytest.mark.parametrize("lens", [[600], [300, 1, 77, 256], [129, 130, 0, 700], [26] * 20], ids=str)
+@pytest.mark.parametrize("nh,nkv,hd", [(148, 148, 128), (100, 50, 64), (160, 32, 128), (120, 40, 80)])
+def test_enough_heads_to_fill_every_sm(nh, nkv, hd, lens):
+    """Two tiles to a block, the second partly or wholly empty."""
+    g = _gen(nh * hd + len(lens))
+    n = sum(lens)
+    q, k, v = _n(g, n, nh, hd, by=1.5), _n(g, n, nkv, hd), _n(g, n, nkv, hd)
+    k[lens[0] - 1] = 0
+    v[lens[0] - 1, :, :9] = float("inf")  # the first sequence's last value
+    got = _ops().prompt_attention(q, k, v, _cu(lens), hd ** -0.5)
+    R.check(got, *R.prompt(q, k, v, _cu(lens), hd ** -0.5)[:2])
+
+
+def test_many_sequences():
+    """More sequences than a warp has lanes, empty ones among them."""
+    g = _gen(70)
+    lens = torch.randint(0, 90, (131,), device=DEV, generator=g).tolist()
+    lens[5], lens[77], lens[130] = 0, 400, 300
+    n = sum(lens)
+    for nh, nkv, hd in ((8, 8, 64), (2, 1, 64)):
+        q, k, v = _n(g, n, nh, hd, by=1.5), _n(g, n, nkv, hd), _n(g, n, nkv, hd)
+        got = _ops().prompt_attention(q, k, v, _cu(lens), hd ** -0.5)
+        R.check(got, *R.prompt(q, k, v, _cu(lens), hd ** -0.5)[:2])
+
+
 @pytest.mark.parametrize("lens,ctx", [([1], [0]), ([64], [500]), ([130, 3], [1, 700]), ([7, 200, 31], [0, 129, 1000])])
 @pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (5, 1, 128), (4, 2, 64), (6, 2, 36)])
 def test_prompts_over_caches(nh, nkv, hd, lens, ctx):
@@ -188,6 +213,18 @@ def test_wide_trees_and_random_masks(t, cols, pos):
     qt = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)  # heads outside the tokens
     out = torch.empty(t, b, nh, hd, device=DEV, dtype=BF).transpose(0, 1)
     R.check(_ops().tree_attention(qt, k, v, _i(p), mask, 0.1, out=out), want, size)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,t", [(40, 8, 128, 60), (16, 16, 64, 200), (16, 8, 128, 130)])
+def test_a_batch_of_wide_trees(nh, nkv, hd, t):
+    """Enough work for two tiles to a block."""
+    g = _gen(t)
+    b, rows = 20, 500
+    pos = torch.randint(0, rows - t, (b,), device=DEV, generator=g)
+    q, k, v = _n(g, b, t, nh, hd, by=1.5), _n(g, b, nkv, rows, hd), _n(g, b, nkv, rows, hd)
+    mask = torch.rand(b, t, t, device=DEV, generator=g) < 0.2
+    want, size = R.tree(q, k, v, pos.tolist(), mask, hd ** -0.5)
+    R.check(_ops().tree_attention(q, k, v, pos, mask, hd ** -0.5), want, size)
 
 
 def test_a_tree_row_that_sees_nothing_is_zero():
