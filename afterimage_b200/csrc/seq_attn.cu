@@ -33,37 +33,40 @@ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { 
 // One sequence: where its queries and keys are and what its rows see. Every
 // value is cut to the extents that the host checked, so that lengths on the
 // device cannot lead outside a tensor.
+// (32 bits: the host limits tokens, sequences and key rows; only offsets in memory need more.)
 struct Seq {
-  int64_t q0, m;    // first query row (within the q batch of a tree: 0) and number of queries
-  int64_t qb;       // q batch
-  int64_t kb, k0;   // k batch and first key row
-  int64_t L;        // keys
-  int64_t off;      // prompt: row i sees keys < off + i + 1; tree: slot of the drafted column 0 (unclamped)
+  int q0, m;    // first query row (within the q batch of a tree: 0) and number of queries
+  int qb;       // q batch
+  int kb, k0;   // k batch and first key row
+  int L;        // keys
+  int off;      // prompt: row i sees keys < off + i + 1; tree: slot of the drafted column 0
 };
 
-__device__ __forceinline__ Seq sequence(const aib_attn_desc &p, int64_t b) {
+__device__ __forceinline__ int cut(int64_t v, int64_t lo, int64_t hi) { return static_cast<int>(clamp64(v, lo, hi)); }
+
+__device__ __forceinline__ Seq sequence(const aib_attn_desc &p, int b) {
   Seq s;
   if (p.mask) {
     s.q0 = 0;
-    s.m = p.tokens;
+    s.m = static_cast<int>(p.tokens);
     s.qb = s.kb = b;
     s.k0 = 0;
     // a position outside [-columns, rows] means nothing more than its end of that range
-    s.off = clamp64(p.pos[b], -p.mask_cols, p.key_rows);
-    s.L = clamp64(s.off + p.mask_cols, 0, p.key_rows);
+    s.off = cut(p.pos[b], -p.mask_cols, p.key_rows);
+    s.L = cut(s.off + p.mask_cols, 0, p.key_rows);
     return s;
   }
-  s.q0 = clamp64(p.cu_q[b], 0, p.tokens);
-  s.m = clamp64(p.cu_q[b + 1], s.q0, p.tokens) - s.q0;
+  s.q0 = cut(p.cu_q[b], 0, p.tokens);
+  s.m = cut(p.cu_q[b + 1], s.q0, p.tokens) - s.q0;
   s.qb = 0;
   if (p.len_k) {
     s.kb = b;
     s.k0 = 0;
-    s.L = clamp64(p.len_k[b], 0, p.key_rows);
+    s.L = cut(p.len_k[b], 0, p.key_rows);
   } else {
     s.kb = 0;
-    s.k0 = clamp64(p.cu_k[b], 0, p.key_rows);
-    s.L = clamp64(p.cu_k[b + 1], s.k0, p.key_rows) - s.k0;
+    s.k0 = cut(p.cu_k[b], 0, p.key_rows);
+    s.L = cut(p.cu_k[b + 1], s.k0, p.key_rows) - s.k0;
   }
   s.off = s.L - s.m;
   return s;
@@ -75,7 +78,7 @@ __device__ __forceinline__ bool sees(const aib_attn_desc &p, const Seq &s, int64
   if (j < s.off) return true;
   const int64_t c = j - s.off;
   return c < p.mask_cols &&
-         p.mask[s.qb * p.mask_batch_stride + i * p.mask_row_stride + c * p.mask_col_stride] != 0;
+         p.mask[static_cast<int64_t>(s.qb) * p.mask_batch_stride + i * p.mask_row_stride + c * p.mask_col_stride] != 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -100,10 +103,10 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
   Seq s;
   int64_t i;
   if (p.mask) {
-    s = sequence(p, tok / p.tokens);
+    s = sequence(p, static_cast<int>(tok / p.tokens));
     i = tok % p.tokens;
   } else {
-    int64_t b = 0;
+    int b = 0;
     while (b < p.batch && p.cu_q[b + 1] <= tok) ++b;
     if (b == p.batch) return;  // behind the last sequence: left as it is
     s = sequence(p, b);
@@ -223,19 +226,15 @@ struct TcParams {
 // What one CTA works on.
 struct Item {
   Seq s;
-  int64_t t0;          // first token of tile 0 within the sequence
-  int cnt[2];          // tokens in each tile
-  int64_t end[2];      // keys that some row of the tile sees lie before this
-  int64_t low[2];      // every row of the tile sees the keys before this
+  int t0;              // first token of tile 0 within the sequence
+  int cnt0, cnt1;      // tokens in each tile
+  int end0, end1;      // keys that some row of the tile sees lie before this
+  int low0, low1;      // every row of the tile sees the keys before this
   int ta, tb;          // key tiles of this share
   bool live;
 };
 
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
 // Item number -> sequence and first tile. Prompts: items are numbered from
 // the last tiles of the longest prompts down (they see the most keys; the
@@ -243,43 +242,40 @@ __device__ __forceinline__ int64_t warp_sum(int64_t v) {
 // in sequence b, the items at level l (the l-th of their sequence) or above
 // are F(l) = sum_b max(0, P_b - l); a binary search finds the item's level.
 // Collective over the warp.
-__device__ __forceinline__ bool find_item(const TcParams &p, int64_t item, int64_t &b, int64_t &level) {
-  const int64_t unit = static_cast<int64_t>(p.tt) * p.tpi;
-  const int64_t batch = p.d.batch;
+__device__ __forceinline__ bool find_item(const TcParams &p, int item, int &b, int &level) {
+  const int unit = p.tt * p.tpi;
+  const int batch = static_cast<int>(p.d.batch), tokens = static_cast<int>(p.d.tokens);
   if (p.d.mask) {
-    const int64_t per = (p.d.tokens + unit - 1) / unit;
+    const int per = (tokens + unit - 1) / unit;
     b = item / per;
     level = item - b * per;
     return b < batch;
   }
   const int lane = threadIdx.x & 31;
-  const auto items_of = [&](int64_t i) {
-    const int64_t q0 = clamp64(p.d.cu_q[i], 0, p.d.tokens);
-    return (clamp64(p.d.cu_q[i + 1], q0, p.d.tokens) - q0 + unit - 1) / unit;
+  const auto items_of = [&](int i) {
+    const int q0 = cut(p.d.cu_q[i], 0, tokens);
+    return (cut(p.d.cu_q[i + 1], q0, tokens) - q0 + unit - 1) / unit;
   };
   if (batch == 1) {
     b = 0;
     level = items_of(0) - 1 - item;
     return level >= 0;
   }
-  const int64_t first = lane < batch ? items_of(lane) : 0;  // the common case needs no second read
-  const auto at_or_above = [&](int64_t l) {
-    int64_t f = first > l ? first - l : 0;
-    for (int64_t i = lane + 32; i < batch; i += 32) {
-      const int64_t n = items_of(i);
-      if (n > l) f += n - l;
-    }
+  const int first = lane < batch ? items_of(lane) : 0;  // the common case needs no second read
+  const auto at_or_above = [&](int l) {
+    int f = max(0, first - l);
+    for (int i = lane + 32; i < batch; i += 32) f += max(0, items_of(i) - l);
     return warp_sum(f);
   };
   if (at_or_above(0) <= item) return false;
-  int64_t lo = 0, hi = (p.d.tokens + unit - 1) / unit;  // F(lo) > item >= F(hi)
+  int lo = 0, hi = (tokens + unit - 1) / unit;  // F(lo) > item >= F(hi)
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
+    const int mid = (lo + hi) >> 1;
     if (at_or_above(mid) > item) lo = mid; else hi = mid;
   }
-  int64_t rank = item - at_or_above(lo + 1);  // among the sequences that reach this level
-  for (int64_t i0 = 0; i0 < batch; i0 += 32) {
-    const int64_t i = i0 + lane;
+  int rank = item - at_or_above(lo + 1);  // among the sequences that reach this level
+  for (int i0 = 0; i0 < batch; i0 += 32) {
+    const int i = i0 + lane;
     unsigned has = __ballot_sync(0xffffffffu, i < batch && (i0 == 0 ? first : items_of(i)) > lo);
     if (rank < __popc(has)) {
       for (; rank > 0; --rank) has &= has - 1;
@@ -292,29 +288,24 @@ __device__ __forceinline__ bool find_item(const TcParams &p, int64_t item, int64
   return false;
 }
 
-__device__ __forceinline__ Item make_item(const TcParams &p, int64_t item, int split) {
+__device__ __forceinline__ void make_tile(const TcParams &p, const Seq &s, int t, bool used, int &cnt, int &end,
+                                          int &low) {
+  cnt = used ? max(0, min(p.tt, s.m - t)) : 0;
+  end = p.d.mask ? s.L : max(0, min(s.off + t + cnt, s.L));
+  low = max(0, min(p.d.mask ? s.off : s.off + t + 1, s.L));
+  if (cnt == 0) end = 0;
+}
+
+__device__ __forceinline__ Item make_item(const TcParams &p, int item, int split) {
   Item w;
-  int64_t b = 0, level = 0;
+  int b = 0, level = 0;
   w.live = find_item(p, item, b, level);
   if (!w.live) return w;
   w.s = sequence(p.d, b);
   w.t0 = level * p.tt * p.tpi;
-  int64_t most = 0;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int64_t t = w.t0 + static_cast<int64_t>(s) * p.tt;
-    w.cnt[s] = s < p.tpi ? static_cast<int>(clamp64(w.s.m - t, 0, p.tt)) : 0;
-    if (p.d.mask) {
-      w.end[s] = w.s.L;
-      w.low[s] = clamp64(w.s.off, 0, w.s.L);
-    } else {
-      w.end[s] = clamp64(w.s.off + t + w.cnt[s], 0, w.s.L);
-      w.low[s] = clamp64(w.s.off + t + 1, 0, w.s.L);
-    }
-    if (w.cnt[s] == 0) w.end[s] = 0;
-    most = w.end[s] > most ? w.end[s] : most;
-  }
-  const int tiles = static_cast<int>((most + kTile - 1) / kTile);
+  make_tile(p, w.s, w.t0, true, w.cnt0, w.end0, w.low0);
+  make_tile(p, w.s, w.t0 + p.tt, p.tpi > 1, w.cnt1, w.end1, w.low1);
+  const int tiles = (max(w.end0, w.end1) + kTile - 1) / kTile;
   const int per = (tiles + p.splits - 1) / p.splits;
   w.ta = min(tiles, split * per);
   w.tb = min(tiles, w.ta + per);
@@ -442,35 +433,68 @@ __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80
 // bits of the seen keys among the four 32-key words of key tile t, for this
 // thread's row (token tok of the tile; first token of the tile is ti within
 // the sequence). Collective over the warp for trees.
-__device__ __forceinline__ void seen_words(const TcParams &p, const Item &w, int s, int tok, int warp_tok0,
+__device__ __forceinline__ void seen_words(const TcParams &p, const Seq &s, int t0, int tok, int warp_tok0,
                                            int warp_tok1, int t, uint32_t (&bits)[4]) {
-  const int64_t key0 = static_cast<int64_t>(t) * kTile;
-  const int64_t i = w.t0 + static_cast<int64_t>(s) * p.tt + tok;
+  const int key0 = t * kTile;
   if (!p.d.mask) {
-    const int64_t n = clamp64(w.s.off + i + 1, 0, w.s.L) - key0;
+    const int n = max(0, min(s.off + t0 + tok + 1, s.L)) - key0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int64_t k = n - 32 * c;
-      bits[c] = k >= 32 ? 0xffffffffu : (k <= 0 ? 0u : (1u << static_cast<int>(k)) - 1u);
+      const int k = n - 32 * c;
+      bits[c] = k >= 32 ? 0xffffffffu : (k <= 0 ? 0u : (1u << k) - 1u);
     }
     return;
   }
   const int lane = threadIdx.x & 31;
-  const uint8_t *m = p.d.mask + w.s.qb * p.d.mask_batch_stride;
+  const uint8_t *m = p.d.mask + static_cast<int64_t>(s.qb) * p.d.mask_batch_stride;
 #pragma unroll
   for (int c = 0; c < 4; ++c) bits[c] = 0;
   for (int a = warp_tok0; a <= warp_tok1; ++a) {
-    const uint8_t *row = m + (w.t0 + static_cast<int64_t>(s) * p.tt + a) * p.d.mask_row_stride;
+    const uint8_t *row = m + static_cast<int64_t>(t0 + a) * p.d.mask_row_stride;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int64_t key = key0 + 32 * c + lane;
-      const int64_t col = key - w.s.off;
-      bool seen = key < w.s.L && col < p.d.mask_cols;
+      const int key = key0 + 32 * c + lane;
+      const int64_t col = static_cast<int64_t>(key) - s.off;
+      bool seen = key < s.L && col < p.d.mask_cols;
       if (seen && col >= 0) seen = row[col * p.d.mask_col_stride] != 0;
       const uint32_t word = __ballot_sync(0xffffffffu, seen);
       if (a == tok) bits[c] = word;
     }
   }
+}
+
+// What V held that is not finite (warps 10-11 took it out of the key tiles
+// first .. last - 1 of the stream) and this thread's row sees is added to its
+// row of O: whatever its weight, the sum is not finite there. Rare and slow.
+// Collective over the warp.
+template <int HDP>
+__device__ __forceinline__ void add_not_finite(const TcParams &p, const Seq &s, int t0, int kvh, int tok, int warp_tok0,
+                                            int warp_tok1, int first, int last, int step, uint32_t to) {
+  const uint16_t *v = static_cast<const uint16_t *>(p.d.v) + s.kb * p.d.v_batch_stride + s.k0 * p.d.v_token_stride +
+                      kvh * p.d.v_head_stride;
+#pragma unroll 1
+  for (int c0 = 0; c0 < HDP; c0 += 32) {
+    uint32_t o[32];
+    tmem_ld32(to + c0, o);
+    tmem_wait_ld();
+#pragma unroll 1
+    for (int t = first; t < last; t += step) {
+      uint32_t bits[4];
+      seen_words(p, s, t0, tok, warp_tok0, warp_tok1, t, bits);
+#pragma unroll 1
+      for (int i = 0; i < kTile; ++i) {
+        const int key = t * kTile + i;
+        const uint32_t word = i < 64 ? (i < 32 ? bits[0] : bits[1]) : (i < 96 ? bits[2] : bits[3]);
+        if (key >= s.L || !((word >> (i & 31)) & 1u)) continue;
+        const uint16_t *vr = v + key * p.d.v_token_stride + c0;
+#pragma unroll
+        for (int d = 0; d < 32; ++d)
+          if (c0 + d < p.d.hd && not_finite_bf16(vr[d])) o[d] = __float_as_uint(__uint_as_float(o[d]) + b2f(vr[d]));
+      }
+    }
+    tmem_st32(to + c0, o);
+  }
+  tmem_wait_st();
 }
 
 template <int HDP>
@@ -492,19 +516,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Item w = make_item(p, rest / p.splits, split);
   if (!w.live) return;  // uniform over the CTA: no barrier or tensor memory is held yet
 
-  const bool pair = w.cnt[1] > 0;
-  // pair: key tiles of each stream; solo: the tiles that both take in turn
-  int n[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int e = static_cast<int>((w.end[s] + kTile - 1) / kTile);
-    n[s] = max(0, min(e, w.tb) - w.ta);
-  }
-  const int nk = pair ? max(n[0], n[1]) : n[0];
-  const int my_n[2] = {pair ? n[0] : (nk + 1) / 2, pair ? n[1] : nk / 2};
+  const bool pair = w.cnt1 > 0;
+  // pair: key tiles of each stream (the second tile's tokens are later: they see as many or more);
+  // solo: the tiles that both streams take in turn
+  const int n0 = max(0, min((w.end0 + kTile - 1) / kTile, w.tb) - w.ta);
+  const int nk = pair ? max(n0, min((w.end1 + kTile - 1) / kTile, w.tb) - w.ta) : n0;
   // the first key tile of this share that some row does not see in full
-  const int64_t low = pair ? min(w.low[0], w.low[1]) : w.low[0];
-  const int first_masked = static_cast<int>(max(static_cast<int64_t>(0), low / kTile - w.ta));
+  const int first_masked = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
 
   const uint32_t smem_q = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = smem_q + 2 * C::kSlotBytes;
@@ -535,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = tmem_base;
   const uint32_t tmem_s[2] = {tmem, tmem + 128};
   const uint32_t tmem_o[2] = {tmem + 256, tmem + 384};
@@ -543,205 +562,213 @@ __global__ void __launch_bounds__(kThreads, 1)
   const auto pos_k = [&](int j) { return pair ? 2 * j : (j == 0 ? 0 : 2 * j - 1); };
   const auto pos_v = [&](int j) { return pair ? 2 * j + 1 : (j == nk - 1 ? 2 * nk - 1 : 2 * j + 2); };
 
-  if (warp == 8) {
-    if (lane == 0 && nk > 0) {
-      const int kb = static_cast<int>(w.s.kb), qb = static_cast<int>(w.s.qb);
-      const uint32_t qbar = smem_u32(&bar_q);
-      const uint32_t qbytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(qbar),
-                   "r"(pair ? 2 * qbytes : qbytes)
-                   : "memory");
-      for (int s = 0; s < (pair ? 2 : 1); ++s)
-        for (int h = 0; h < C::kHalves; ++h)
-          tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group,
-                      static_cast<int>(w.s.q0 + w.t0) + s * p.tt, qb, qbar);
-      int issued = 0;
-      for (int pos = 0; pos < 2 * nk; ++pos) {
-        const int slot = pos % C::kSlots;
-        const unsigned ph = static_cast<unsigned>(pos / C::kSlots) & 1u;
-        if (!mbar_wait(smem_u32(&bar_empty[slot]), ph ^ 1u, &gave_up)) break;
-        bool is_v;
-        int j;
-        if (pair) {
-          is_v = pos & 1;
-          j = pos >> 1;
-        } else {
-          is_v = pos > 0 && (pos % 2 == 0 || pos == 2 * nk - 1);
-          j = pos == 0 ? 0 : (pos == 2 * nk - 1 ? nk - 1 : (is_v ? pos / 2 - 1 : (pos + 1) / 2));
-        }
-        const uint32_t fb = smem_u32(&bar_full[slot]);
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"(C::kSlotBytes) : "memory");
-        const int row = static_cast<int>(w.s.k0) + (w.ta + j) * kTile;
-        for (int h = 0; h < C::kHalves; ++h)
-          tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, is_v ? &map_v : &map_k, h * 64, row, kvh, kb, fb);
-        issued = pos + 1;
-      }
-      // copies in flight land before the CTA can end (bounded)
-      (void)mbar_wait(qbar, 0, &gave_up);
-      for (int pos = max(0, issued - C::kSlots); pos < issued; ++pos)
-        for (unsigned k = 0; k < kWaitLimit; ++k) {
-          if (mbar_try(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u)) break;
-          __nanosleep(32);
-        }
-    }
-  } else if (warp == 9) {
-    if (lane == 0 && nk > 0) {
-      constexpr uint32_t id_s = idesc_bf16(kTile, 0), id_o = idesc_bf16(HDP, 1);
-      unsigned clean_ph = 0, p_ph[2] = {0, 0};
-      bool o_open[2] = {false, false};  // has the stream's O been written?
-      bool ok = mbar_wait(smem_u32(&bar_q), 0, &gave_up);
-      const auto wait_full = [&](int pos) {
-        return mbar_wait(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u, &gave_up);
-      };
-      const auto scores = [&](int s, int pos) {  // S of stream s from the K tile at ring position pos
-        const uint32_t q = smem_q + (pair ? s : 0) * C::kSlotBytes, k = ring + (pos % C::kSlots) * C::kSlotBytes;
-#pragma unroll
-        for (int i = 0; i < C::kHalves * 4; ++i) {
-          const uint32_t o = (i / 4) * 16384 + (i % 4) * 32;
-          mma_ss(tmem_s[s], desc_kmajor(q + o), desc_kmajor(k + o), id_s, i > 0);
-        }
-        mma_commit(smem_u32(&bar_s[s]));
-      };
-      const auto values = [&](int s, int pos) {  // O of stream s from its P and the V tile at pos
-        const uint32_t v = ring + (pos % C::kSlots) * C::kSlotBytes;
-#pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-          mma_ts(tmem_o[s], tmem_s[s] + i * 8, desc_mnmajor(v + i * 2048), id_o, (i > 0 || o_open[s]) ? 1u : 0u);
-        o_open[s] = true;
-      };
-      // V tile j has landed; warps 10-11 look it over (while the softmax runs) where some row does not see all of it
-      const auto wait_v = [&](int j, int pos) {
-        if (!wait_full(pos)) return false;
-        if (j >= first_masked) mbar_arrive(smem_u32(&bar_dirty));
-        return true;
-      };
-      const auto wait_clean = [&](int j) {
-        if (j < first_masked) return true;
-        const bool r = mbar_wait(smem_u32(&bar_clean), clean_ph, &gave_up);
-        clean_ph ^= 1u;
-        return r;
-      };
-      const auto wait_p = [&](int s) {
-        const bool r = mbar_wait(smem_u32(&bar_p[s]), p_ph[s], &gave_up);
-        p_ph[s] ^= 1u;
-        return r;
-      };
-      const auto release = [&](int pos) { mma_commit(smem_u32(&bar_empty[pos % C::kSlots])); };
-      if (ok && pair) {
-        ok = wait_full(0);
-        fence_after();
-        if (ok) {
-          if (n[0] > 0) scores(0, 0);
-          scores(1, 0);
-          release(0);
-        }
-        for (int j = 0; ok && j < nk; ++j) {
-          const int pv = pos_v(j), pk = pos_k(j + 1);
-          if (!(ok = wait_v(j, pv))) break;
-          const bool more = j + 1 < nk;
-          if (j < n[0] && !(ok = wait_p(0))) break;
-          if (!(ok = wait_clean(j))) break;
-          if (j < n[0]) {
-            fence_after();
-            values(0, pv);
-            if (j + 1 == n[0]) mma_commit(smem_u32(&bar_o[0]));
-          }
-          if (more) {
-            if (!(ok = wait_full(pk))) break;
-            fence_after();
-            if (j + 1 < n[0]) scores(0, pk);
-          }
-          if (!(ok = wait_p(1))) break;
-          fence_after();
-          values(1, pv);
-          release(pv);
-          if (more) {
-            scores(1, pk);
-            release(pk);
-          } else {
-            mma_commit(smem_u32(&bar_o[1]));
-          }
-        }
-      } else if (ok) {
-        ok = wait_full(0);
-        fence_after();
-        if (ok) {
-          scores(0, 0);
-          release(0);
-        }
-        for (int j = 0; ok && j < nk; ++j) {
-          const int s = j & 1;
-          if (j + 1 < nk) {
-            const int pk = pos_k(j + 1);
-            if (!(ok = wait_full(pk))) break;
-            fence_after();
-            scores(s ^ 1, pk);
-            release(pk);
-          }
-          const int pv = pos_v(j);
-          if (!(ok = wait_v(j, pv)) || !(ok = wait_p(s)) || !(ok = wait_clean(j))) break;
-          fence_after();
-          values(s, pv);
-          release(pv);
-          if (j + 2 >= nk) mma_commit(smem_u32(&bar_o[s]));
-        }
-      }
-      // nothing of this CTA is in flight in the tensor core when it ends
-      mma_commit(smem_u32(&bar_drain));
-      for (unsigned k = 0; k < kWaitLimit && !mbar_try(smem_u32(&bar_drain), 0); ++k) __nanosleep(32);
-    }
-  } else if (warp >= 10) {
-    // ---- V tiles that some row does not see in full: what is not finite becomes zero
-    const int64_t seen_end = w.end[0] > w.end[1] ? w.end[0] : w.end[1];
-    const int self = static_cast<int>(threadIdx.x) - 320;
-    for (int j = first_masked; j < nk; ++j) {
-      if (!warp_wait(smem_u32(&bar_dirty), (j - first_masked) & 1u, &gave_up)) break;
-      const uint32_t base = ring + (pos_v(j) % C::kSlots) * C::kSlotBytes;
-      const int64_t rows_seen = seen_end - static_cast<int64_t>(w.ta + j) * kTile;
-      for (int e = self; e < C::kSlotBytes / 16; e += 64) {
-        uint32_t x[4];
-        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                     : "r"(base + e * 16)
+  // 384 threads start with 168 registers each; the softmax warps take over what the others leave
+  // (256 x 216 + 128 x 72 = 384 x 168)
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      if (lane == 0 && nk > 0) {
+              const uint32_t qbar = smem_u32(&bar_q);
+        const uint32_t qbytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(qbar),
+                     "r"(pair ? 2 * qbytes : qbytes)
                      : "memory");
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (not_finite_bf16(x[i])) x[i] &= 0xffff0000u, found = true;
-          if (not_finite_bf16(x[i] >> 16)) x[i] &= 0x0000ffffu, found = true;
+        for (int s = 0; s < (pair ? 2 : 1); ++s)
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group,
+                        w.s.q0 + w.t0 + s * p.tt, w.s.qb, qbar);
+        int issued = 0;
+        for (int pos = 0; pos < 2 * nk; ++pos) {
+          const int slot = pos % C::kSlots;
+          const unsigned ph = static_cast<unsigned>(pos / C::kSlots) & 1u;
+          if (!mbar_wait(smem_u32(&bar_empty[slot]), ph ^ 1u, &gave_up)) break;
+          bool is_v;
+          int j;
+          if (pair) {
+            is_v = pos & 1;
+            j = pos >> 1;
+          } else {
+            is_v = pos > 0 && (pos % 2 == 0 || pos == 2 * nk - 1);
+            j = pos == 0 ? 0 : (pos == 2 * nk - 1 ? nk - 1 : (is_v ? pos / 2 - 1 : (pos + 1) / 2));
+          }
+          const uint32_t fb = smem_u32(&bar_full[slot]);
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"(C::kSlotBytes) : "memory");
+          const int row = w.s.k0 + (w.ta + j) * kTile;
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, is_v ? &map_v : &map_k, h * 64, row, kvh, w.s.kb, fb);
+          issued = pos + 1;
         }
-        if (found) {
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + e * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
-                       "r"(x[3])
-                       : "memory");
-          if ((e % 1024) / 8 < rows_seen) bad_seen = 1;
-        }
+        // copies in flight land before the CTA can end (bounded)
+        (void)mbar_wait(qbar, 0, &gave_up);
+        for (int pos = max(0, issued - C::kSlots); pos < issued; ++pos)
+          for (unsigned k = 0; k < kWaitLimit; ++k) {
+            if (mbar_try(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u)) break;
+            __nanosleep(32);
+          }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_clean));
+    } else if (warp == 9) {
+      if (lane == 0 && nk > 0) {
+        constexpr uint32_t id_s = idesc_bf16(kTile, 0), id_o = idesc_bf16(HDP, 1);
+        unsigned clean_ph = 0, p_ph[2] = {0, 0};
+        bool o_open[2] = {false, false};  // has the stream's O been written?
+        bool ok = mbar_wait(smem_u32(&bar_q), 0, &gave_up);
+        const auto wait_full = [&](int pos) {
+          return mbar_wait(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u, &gave_up);
+        };
+        const auto scores = [&](int s, int pos) {  // S of stream s from the K tile at ring position pos
+          const uint32_t q = smem_q + (pair ? s : 0) * C::kSlotBytes, k = ring + (pos % C::kSlots) * C::kSlotBytes;
+#pragma unroll
+          for (int i = 0; i < C::kHalves * 4; ++i) {
+            const uint32_t o = (i / 4) * 16384 + (i % 4) * 32;
+            mma_ss(tmem_s[s], desc_kmajor(q + o), desc_kmajor(k + o), id_s, i > 0);
+          }
+          mma_commit(smem_u32(&bar_s[s]));
+        };
+        const auto values = [&](int s, int pos) {  // O of stream s from its P and the V tile at pos
+          const uint32_t v = ring + (pos % C::kSlots) * C::kSlotBytes;
+#pragma unroll
+          for (int i = 0; i < kTile / 16; ++i)
+            mma_ts(tmem_o[s], tmem_s[s] + i * 8, desc_mnmajor(v + i * 2048), id_o, (i > 0 || o_open[s]) ? 1u : 0u);
+          o_open[s] = true;
+        };
+        // V tile j has landed; warps 10-11 look it over (while the softmax runs) where some row does not see all of it
+        const auto wait_v = [&](int j, int pos) {
+          if (!wait_full(pos)) return false;
+          if (j >= first_masked) mbar_arrive(smem_u32(&bar_dirty));
+          return true;
+        };
+        const auto wait_clean = [&](int j) {
+          if (j < first_masked) return true;
+          const bool r = mbar_wait(smem_u32(&bar_clean), clean_ph, &gave_up);
+          clean_ph ^= 1u;
+          return r;
+        };
+        const auto wait_p = [&](int s) {
+          const bool r = mbar_wait(smem_u32(&bar_p[s]), p_ph[s], &gave_up);
+          p_ph[s] ^= 1u;
+          return r;
+        };
+        const auto release = [&](int pos) { mma_commit(smem_u32(&bar_empty[pos % C::kSlots])); };
+        if (ok && pair) {
+          ok = wait_full(0);
+          fence_after();
+          if (ok) {
+            if (n0 > 0) scores(0, 0);
+            scores(1, 0);
+            release(0);
+          }
+          for (int j = 0; ok && j < nk; ++j) {
+            const int pv = pos_v(j), pk = pos_k(j + 1);
+            if (!(ok = wait_v(j, pv))) break;
+            const bool more = j + 1 < nk;
+            if (j < n0 && !(ok = wait_p(0))) break;
+            if (!(ok = wait_clean(j))) break;
+            if (j < n0) {
+              fence_after();
+              values(0, pv);
+              if (j + 1 == n0) mma_commit(smem_u32(&bar_o[0]));
+            }
+            if (more) {
+              if (!(ok = wait_full(pk))) break;
+              fence_after();
+              if (j + 1 < n0) scores(0, pk);
+            }
+            if (!(ok = wait_p(1))) break;
+            fence_after();
+            values(1, pv);
+            release(pv);
+            if (more) {
+              scores(1, pk);
+              release(pk);
+            } else {
+              mma_commit(smem_u32(&bar_o[1]));
+            }
+          }
+        } else if (ok) {
+          ok = wait_full(0);
+          fence_after();
+          if (ok) {
+            scores(0, 0);
+            release(0);
+          }
+          for (int j = 0; ok && j < nk; ++j) {
+            const int s = j & 1;
+            if (j + 1 < nk) {
+              const int pk = pos_k(j + 1);
+              if (!(ok = wait_full(pk))) break;
+              fence_after();
+              scores(s ^ 1, pk);
+              release(pk);
+            }
+            const int pv = pos_v(j);
+            if (!(ok = wait_v(j, pv)) || !(ok = wait_p(s)) || !(ok = wait_clean(j))) break;
+            fence_after();
+            values(s, pv);
+            release(pv);
+            if (j + 2 >= nk) mma_commit(smem_u32(&bar_o[s]));
+          }
+        }
+        // nothing of this CTA is in flight in the tensor core when it ends
+        mma_commit(smem_u32(&bar_drain));
+        for (unsigned k = 0; k < kWaitLimit && !mbar_try(smem_u32(&bar_drain), 0); ++k) __nanosleep(32);
+      }
+    } else {
+      // ---- V tiles that some row does not see in full: what is not finite becomes zero
+      const int seen_end = max(w.end0, w.end1);
+      const int self = static_cast<int>(threadIdx.x) - 320;
+      for (int j = first_masked; j < nk; ++j) {
+        if (!warp_wait(smem_u32(&bar_dirty), (j - first_masked) & 1u, &gave_up)) break;
+        const uint32_t base = ring + (pos_v(j) % C::kSlots) * C::kSlotBytes;
+        const int rows_seen = seen_end - (w.ta + j) * kTile;
+#pragma unroll 4
+        for (int e = self; e < C::kSlotBytes / 16; e += 64) {
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(base + e * 16)
+                       : "memory");
+          bool found = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (not_finite_bf16(x[i])) x[i] &= 0xffff0000u, found = true;
+            if (not_finite_bf16(x[i] >> 16)) x[i] &= 0x0000ffffu, found = true;
+          }
+          if (found) {
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + e * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                         "r"(x[3])
+                         : "memory");
+            if ((e % 1024) / 8 < rows_seen) bad_seen = 1;
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_clean));
+      }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax: one thread per row of the stream's tile
     const int s = warp >> 2;
     const int tile = pair ? s : 0;
+    const int cnt = tile ? w.cnt1 : w.cnt0, low = tile ? w.low1 : w.low0;
+    const int t0 = w.t0 + tile * p.tt;  // first token of the tile
     const int wrow = (warp & 3) * 32, row = wrow + lane;
-    const int rows = w.cnt[tile] * p.group;
+    const int rows = cnt * p.group;
     const bool active = wrow < rows;  // a warp without rows only keeps the barriers going
-    const int tok = min(row / p.group, w.cnt[tile] - 1);
-    const int tok0 = wrow / p.group, tok1 = min((wrow + 31) / p.group, w.cnt[tile] - 1);
+    const int tok = min(row / p.group, cnt - 1);
+    const int tok0 = wrow / p.group, tok1 = min((wrow + 31) / p.group, cnt - 1);
     const uint32_t lanes = static_cast<uint32_t>(wrow) << 16;
     const uint32_t ts = tmem_s[s] + lanes, to = tmem_o[s] + lanes;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
-    const int mine = my_n[s];
+    const int mine = pair ? (s ? nk : n0) : (nk + 1 - s) / 2;
     bool ok = true;
     for (int it = 0; it < mine; ++it) {
       const int j = pair ? it : 2 * it + s;
       const int t = w.ta + j;
-      const bool masked = (static_cast<int64_t>(t) + 1) * kTile > w.low[tile];
+      const bool masked = (t + 1) * kTile > low;
       uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      if (masked && active) seen_words(p, w, tile, tok, tok0, tok1, t, bits);
+      if (masked && active) seen_words(p, w.s, t0, tok, tok0, tok1, t, bits);
       if (!(ok = warp_wait(smem_u32(&bar_s[s]), it & 1, &gave_up))) break;
       fence_after();
       if (active) {
@@ -801,28 +828,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && mine > 0) ok = warp_wait(smem_u32(&bar_o[s]), 0, &gave_up);
     fence_after();
 
-    // what V held that is not finite and this row sees, in one column block
-    const auto add_bad = [&](float *o, int c0) {
-      const uint16_t *v = static_cast<const uint16_t *>(p.d.v) + w.s.kb * p.d.v_batch_stride +
-                          w.s.k0 * p.d.v_token_stride + kvh * p.d.v_head_stride;
-      for (int it = 0; it < mine; ++it) {
-        const int j = pair ? it : 2 * it + s;
-        if (j < first_masked) continue;
-        uint32_t bits[4];
-        seen_words(p, w, tile, tok, tok0, tok1, w.ta + j, bits);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          for (int i = 0; i < 32; ++i) {
-            const int64_t key = static_cast<int64_t>(w.ta + j) * kTile + 32 * c + i;
-            if (key >= w.s.L || !((bits[c] >> i) & 1u)) continue;
-            const uint16_t *vr = v + key * p.d.v_token_stride;
-#pragma unroll
-            for (int d = 0; d < 32; ++d)
-              if (c0 + d < p.d.hd && not_finite_bf16(vr[c0 + d])) o[d] += b2f(vr[c0 + d]);
-          }
-      }
-    };
-    const bool fix = __any_sync(0xffffffffu, *static_cast<volatile int *>(&bad_seen) != 0);
+    if (mine > 0 && active && ok && __any_sync(0xffffffffu, *static_cast<volatile int *>(&bad_seen) != 0)) {
+      const int step = pair ? 1 : 2;
+      int first = pair ? 0 : s;
+      if (first < first_masked) first += (first_masked - first + step - 1) / step * step;
+      add_not_finite<HDP>(p, w.s, t0, kvh, tok, tok0, tok1, w.ta + first, w.ta + (pair ? mine : nk), step, to);
+    }
     float *joined = reinterpret_cast<float *>(raw + (ring - smem_u32(raw)));  // [HDP][128], over the ring
 
     if (!pair) {
@@ -837,7 +848,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t o[32];
             tmem_ld32(to + 32 * c, o);
             tmem_wait_ld();
-            if (fix) add_bad(reinterpret_cast<float *>(o), 32 * c);
 #pragma unroll
             for (int i = 0; i < 32; ++i) joined[(32 * c + i) * kTile + row] = __uint_as_float(o[i]);
           }
@@ -846,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if ((pair || s == 0) && active && ok) {
       float a0 = 1.f, a1 = 0.f;
-      const bool second = !pair && my_n[1] > 0;
+      const bool second = !pair && nk > 1;
       if (second) {
         const float m1 = join[0][row], mm = fmaxf(m, m1);
         const float ref = mm == -INFINITY ? 0.f : mm;
@@ -859,16 +869,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       const int64_t unit = (static_cast<int64_t>(rest) * p.d.nkv + kvh) * p.tpi + tile;
       float *part = p.d.workspace + unit * (kTile * (HDP + 2));
-      const int64_t token = w.s.q0 + w.t0 + static_cast<int64_t>(tile) * p.tt + tok;
+      const int64_t token = w.s.q0 + t0 + tok;
       uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
-                      (kvh * p.group + row % p.group) * p.d.out_head_stride;
+                      static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
 #pragma unroll
       for (int c = 0; c < HDP / 32; ++c) {
         float o[32];
         if (mine > 0) {
           tmem_ld32(to + 32 * c, reinterpret_cast<uint32_t *>(o));
           tmem_wait_ld();
-          if (fix) add_bad(o, 32 * c);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
@@ -912,46 +921,60 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the shares of the key axis: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
-// A block takes 32 rows of one tile, a warp 8 of their columns.
+// A block takes 32 rows of one tile: the weights of all shares first, then a
+// warp for 8 columns, a lane for a row.
+constexpr int kMaxSplits = 64;
+
 template <int HDP>
 __global__ void __launch_bounds__(HDP * 4) attn_join_kernel(const __grid_constant__ TcParams p) {
+  __shared__ float weight[kMaxSplits][32], sums[kMaxSplits][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t u = blockIdx.x;
-  const int quarter = static_cast<int>(u % 4);
+  int u = blockIdx.x;
+  const int quarter = u % 4;
   u /= 4;
-  const int tile = static_cast<int>(u % p.tpi);
+  const int tile = u % p.tpi;
   u /= p.tpi;
-  const int kvh = static_cast<int>(u % p.d.nkv);
-  const int64_t item = u / p.d.nkv;
+  const int kvh = u % p.d.nkv;
+  const int item = u / p.d.nkv;
   const Item w = make_item(p, item, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!w.live) return;
+  const int rows = (tile ? w.cnt1 : w.cnt0) * p.group;
+  if (quarter * 32 >= rows) return;
   const int row = quarter * 32 + lane;
-  if (row >= w.cnt[tile] * p.group) return;
-  const int c0 = warp * 8;
-  if (c0 >= p.d.hd) return;
-  const auto part = [&](int sp) {
-    return p.d.workspace + (((item * p.splits + sp) * p.d.nkv + kvh) * p.tpi + tile) * (kTile * (HDP + 2));
-  };
-  // a share that the item's key tiles do not reach holds nothing: the CTA wrote a sum of zero there
-  float m = -INFINITY;
-  for (int sp = 0; sp < p.splits; ++sp) m = fmaxf(m, part(sp)[HDP * kTile + row]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[8] = {};
-  for (int sp = 0; sp < p.splits; ++sp) {
-    const float *q = part(sp);
-    const float ls = q[(HDP + 1) * kTile + row];
-    if (ls == 0.f) continue;
-    const float a = ex2(q[HDP * kTile + row] - ref);
-    l += a * ls;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] += a * q[(c0 + i) * kTile + row];
+  const bool valid = row < rows;
+  const int64_t share = static_cast<int64_t>(p.d.nkv) * p.tpi * (kTile * (HDP + 2));
+  const float *part = p.d.workspace + (static_cast<int64_t>(item) * p.splits * p.d.nkv * p.tpi + kvh * p.tpi + tile) *
+                                          (kTile * (HDP + 2));
+  for (int sp = warp; sp < p.splits; sp += HDP / 8) {
+    weight[sp][lane] = valid ? part[sp * share + HDP * kTile + row] : -INFINITY;
+    sums[sp][lane] = valid ? part[sp * share + (HDP + 1) * kTile + row] : 0.f;
   }
+  __syncthreads();
+  float m = -INFINITY;
+  for (int sp = 0; sp < p.splits; ++sp) m = fmaxf(m, weight[sp][lane]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  const int c0 = warp * 8;
+  float l = 0.f, o[8] = {};
+#pragma unroll 4
+  for (int sp = 0; sp < p.splits; ++sp) {
+    const float ls = sums[sp][lane];
+    // a share that the row's keys do not reach has a sum of zero and no O
+    const bool some = ls != 0.f && c0 < p.d.hd;
+    const float a = some ? ex2(weight[sp][lane] - ref) : 0.f;
+    l += a * ls;
+    const float *q = part + sp * share + c0 * kTile + row;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] += a * (some ? q[i * kTile] : 0.f);
+  }
+  if (!valid || c0 >= p.d.hd) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] *= inv;
-  const int64_t token = w.s.q0 + w.t0 + static_cast<int64_t>(tile) * p.tt + row / p.group;
+  const int tok = row / p.group;
+  const int64_t token = w.s.q0 + w.t0 + tile * p.tt + tok;
   uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
-                  (kvh * p.group + row % p.group) * p.d.out_head_stride + c0;
+                  static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride + c0;
   if (p.vec_out) {
     *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]),
                                                  pack_bf16(o[6], o[7]));
@@ -972,9 +995,9 @@ static int check_common(const aib_attn_desc *p, const char *who) {
     return aib_set_errorf("%s: bad shape (tokens %lld, batch %lld, key rows %lld, heads %d / %d, head size %d of at "
                           "most %d)", who, (long long)p->tokens, (long long)p->batch, (long long)p->key_rows, p->nh,
                           p->nkv, p->hd, kPlainMaxHd), AIB_EINVAL;
-  const int64_t big = INT32_MAX;
+  const int64_t big = INT32_MAX - 1024;  // room for a tile behind the last row
   if (p->tokens > big || p->batch > big || p->key_rows > big)
-    return aib_set_errorf("%s: tokens, batch and key rows must fit in 32 bits", who), AIB_EINVAL;
+    return aib_set_errorf("%s: tokens, batch and key rows must be below 2^31 - 1024", who), AIB_EINVAL;
   if (!std::isfinite(p->scale)) return aib_set_errorf("%s: scale is not finite", who), AIB_EINVAL;
   return AIB_OK;
 }
@@ -1057,7 +1080,7 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
     const int64_t units = std::max<int64_t>(1, pl.items * d.nkv);
     // shares of at least two key tiles (one for each stream), at most one CTA per SM
     const int64_t tiles = (d.key_rows + kTile - 1) / kTile;
-    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, (tiles + 1) / 2)));
+    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / units, (tiles + 1) / 2), kMaxSplits)));
   }
   return pl;
 }
@@ -1109,8 +1132,17 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   const int64_t grid = pl.items * pl.splits * d.nkv;
   attn_tc_kernel<HDP><<<static_cast<unsigned>(grid), kThreads, Cfg<HDP>::kSmem, st>>>(mq, mk, mv, p);
   if ((e = cudaGetLastError()) == cudaSuccess && pl.splits > 1) {
-    attn_join_kernel<HDP><<<static_cast<unsigned>(pl.items * d.nkv * pl.tpi * 4), HDP * 4, 0, st>>>(p);
-    e = cudaGetLastError();
+    // started while the last shares still run (it waits for them before it reads)
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(pl.items * d.nkv * pl.tpi * 4));
+    cfg.blockDim = dim3(HDP * 4);
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attn_join_kernel<HDP>, p);
   }
   if (e != cudaSuccess) return aib_set_errorf("%s: %s", who, cudaGetErrorString(e)), AIB_ECUDA;
   return AIB_OK;
