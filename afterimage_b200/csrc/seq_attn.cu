@@ -226,6 +226,7 @@ struct TcParams {
 // What one CTA works on.
 struct Item {
   Seq s;
+  int shares;          // shares of the key axis that hold any of the item's key tiles
   int t0;              // first token of tile 0 within the sequence
   int cnt0, cnt1;      // tokens in each tile
   int end0, end1;      // keys that some row of the tile sees lie before this
@@ -307,6 +308,7 @@ __device__ __forceinline__ Item make_item(const TcParams &p, int item, int split
   make_tile(p, w.s, w.t0 + p.tt, p.tpi > 1, w.cnt1, w.end1, w.low1);
   const int tiles = (max(w.end0, w.end1) + kTile - 1) / kTile;
   const int per = (tiles + p.splits - 1) / p.splits;
+  w.shares = per ? (tiles + per - 1) / per : 0;
   w.ta = min(tiles, split * per);
   w.tb = min(tiles, w.ta + per);
   return w;
@@ -320,6 +322,9 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, unsigned count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ bool mbar_try(uint32_t bar, unsigned parity) {
   uint32_t ok;
   asm volatile(
@@ -329,23 +334,30 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, unsigned parity) {
       : "memory");
   return ok != 0;
 }
-// true when the phase of `parity` completed within the bound; gives up early when another role did
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, unsigned parity, volatile int *gave_up) {
+// Waits, as a whole warp, for the phase of `parity`; false when the bound is
+// reached or another role gave up. One answer for all lanes: what follows
+// stays uniform, which the warp-wide instructions need and the issue of the
+// matrix and copy instructions (their operands are uniform registers) is
+// faster for.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, unsigned parity, volatile int *gave_up) {
   for (unsigned n = 0; n < kWaitLimit; ++n) {
-    if (mbar_try(bar, parity)) return true;
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
     if (n > 256) {
-      if (*gave_up) break;
+      if (__any_sync(0xffffffffu, *gave_up)) break;
       __nanosleep(32);
     }
   }
   *gave_up = 1;
   return false;
 }
-
-// the same for a whole warp: one answer, so that its lanes stay together
-__device__ __forceinline__ bool warp_wait(uint32_t bar, unsigned parity, volatile int *gave_up) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up));
+// one lane of a converged warp
+__device__ __forceinline__ bool elect() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes != 0;
 }
+// a value that is the same in all lanes, known to be so
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w,
                                             uint32_t bar) {
@@ -358,12 +370,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 // shared-memory matrix descriptors, 128-byte swizzle. K-major (Q, K): 128-byte
 // rows, 8-row groups 1024 bytes apart. MN-major (V, rows are keys): 64 columns
 // a block, blocks of 64 columns 16 KiB apart, 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_base(uint32_t addr, uint64_t lead) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (lead << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) { return desc_base(addr, 1); }
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) { return desc_base(addr, 16384 >> 4); }
+// Only the low word differs between tiles: it holds address / 16, so that a
+// step inside a tile is one addition. (One thread issues every matrix
+// instruction of the CTA, between softmax warps that keep its scheduler busy:
+// with the descriptors built for each instruction it was what the 16384-token
+// prompt waited for.)
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return addr >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mnmajor(uint32_t addr) { return addr >> 4 | (16384u >> 4) << 16; }
 
 // BF16 x BF16 -> F32, M = 128
 __host__ __device__ constexpr uint32_t idesc_bf16(int n, int b_mn_major) {
@@ -371,16 +385,19 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int n, int b_mn_major) {
          (static_cast<uint32_t>(n >> 3) << 17) | ((kTile >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// descriptors by their low words; `acc` 0: the first of a sum
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
@@ -428,6 +445,54 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// two floats side by side, for the packed fp32 instructions
+__device__ __forceinline__ uint64_t two(uint32_t lo, uint32_t hi) {
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint64_t two(float v) { return two(__float_as_uint(v), __float_as_uint(v)); }
+__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^t for two t <= 8 on the multiply-add pipe, beside the exponential unit
+// (16 results a clock and SM, which 128 x 128 weights would keep busy as long
+// as the tensor core takes for a tile). t = r + f with r the nearest integer
+// (the sum with 1.5 2^23 leaves it in the low mantissa bits) and |f| <= 1/2;
+// 2^f by the cubic 1 + f (c1 + f (c2 + f c3)) of least relative error on that
+// interval (fitted as a linear program; 1.0e-4, a fortieth of the BF16 step
+// that P is rounded to); r goes into the exponent. t is held at -127, where the cubic is
+// 1 and the exponent comes to nothing: masked scores give 0 exactly.
+__device__ __forceinline__ void exp2_poly(uint64_t t, float &e0, float &e1) {
+  t = two(__float_as_uint(fmaxf(low_of(t), -127.f)), __float_as_uint(fmaxf(high_of(t), -127.f)));
+  const uint64_t r = add2(t, two(12582912.f));
+  const uint64_t f = fma2(add2(r, two(-12582912.f)), two(-1.f), t);
+  uint64_t y = fma2(two(0.055009059607982635f), f, two(0.2422109693288803f));
+  y = fma2(y, f, two(0.6932829022407532f));
+  y = fma2(y, f, two(1.f));
+  e0 = __uint_as_float((static_cast<uint32_t>(r) << 23) + static_cast<uint32_t>(y));
+  e1 = __uint_as_float((static_cast<uint32_t>(r >> 32) << 23) + static_cast<uint32_t>(y >> 32));
+}
+// of every kPolyOf pairs of weights, kPoly take the polynomial
+constexpr int kPoly = 0, kPolyOf = 8;
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 
 // bits of the seen keys among the four 32-key words of key tile t, for this
@@ -509,21 +574,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int gave_up, bad_seen;
   __shared__ float join[2][kTile];  // maximum and sum of stream 1's rows
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.d.nkv;
   const int rest = blockIdx.x / p.d.nkv;
   const int split = rest % p.splits;
-  const Item w = make_item(p, rest / p.splits, split);
-  if (!w.live) return;  // uniform over the CTA: no barrier or tensor memory is held yet
-
-  const bool pair = w.cnt1 > 0;
-  // pair: key tiles of each stream (the second tile's tokens are later: they see as many or more);
-  // solo: the tiles that both streams take in turn
-  const int n0 = max(0, min((w.end0 + kTile - 1) / kTile, w.tb) - w.ta);
-  const int nk = pair ? max(n0, min((w.end1 + kTile - 1) / kTile, w.tb) - w.ta) : n0;
-  // the first key tile of this share that some row does not see in full
-  const int first_masked = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
-
   const uint32_t smem_q = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = smem_q + 2 * C::kSlotBytes;
 
@@ -545,21 +599,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     bad_seen = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 8 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+  }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
   }
+  const Item w = make_item(p, rest / p.splits, split);
+
+  const bool pair = w.live && w.cnt1 > 0;
+  // pair: key tiles of each stream (the second tile's tokens are later: they see as many or more);
+  // solo: the tiles that both streams take in turn
+  const int n0 = !w.live ? 0 : max(0, min((w.end0 + kTile - 1) / kTile, w.tb) - w.ta);
+  const int nk = !w.live ? 0 : pair ? max(n0, min((w.end1 + kTile - 1) / kTile, w.tb) - w.ta) : n0;
+  // the first key tile of this share that some row does not see in full
+  const int first_masked = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
+
+  const int pairs = uniform(pair), n_k = uniform(nk), n_0 = uniform(n0), n_full = uniform(first_masked);
   __syncthreads();
   fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const uint32_t tmem = tmem_base;
-  const uint32_t tmem_s[2] = {tmem, tmem + 128};
-  const uint32_t tmem_o[2] = {tmem + 256, tmem + 384};
+  // the whole tensor memory is taken, so it starts at column 0: S (and P) of stream s at 128 s, O at 256 + 128 s
 
-  // ring positions of the K and V tiles, in the order in which the matrix instructions want them
-  const auto pos_k = [&](int j) { return pair ? 2 * j : (j == 0 ? 0 : 2 * j - 1); };
+  // The ring holds the tiles in the order in which the matrix instructions want them: K0 V0 K1 V1 ... for a pair,
+  // K0 K1 V0 K2 V1 ... solo.
   const auto pos_v = [&](int j) { return pair ? 2 * j + 1 : (j == nk - 1 ? 2 * nk - 1 : 2 * j + 2); };
 
   // 384 threads start with 168 registers each; the softmax warps take over what the others leave
@@ -567,150 +635,160 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
-      if (lane == 0 && nk > 0) {
-              const uint32_t qbar = smem_u32(&bar_q);
-        const uint32_t qbytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(qbar),
-                     "r"(pair ? 2 * qbytes : qbytes)
-                     : "memory");
-        for (int s = 0; s < (pair ? 2 : 1); ++s)
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group,
-                        w.s.q0 + w.t0 + s * p.tt, w.s.qb, qbar);
-        int issued = 0;
-        for (int pos = 0; pos < 2 * nk; ++pos) {
-          const int slot = pos % C::kSlots;
-          const unsigned ph = static_cast<unsigned>(pos / C::kSlots) & 1u;
-          if (!mbar_wait(smem_u32(&bar_empty[slot]), ph ^ 1u, &gave_up)) break;
-          bool is_v;
-          int j;
-          if (pair) {
-            is_v = pos & 1;
-            j = pos >> 1;
-          } else {
-            is_v = pos > 0 && (pos % 2 == 0 || pos == 2 * nk - 1);
-            j = pos == 0 ? 0 : (pos == 2 * nk - 1 ? nk - 1 : (is_v ? pos / 2 - 1 : (pos + 1) / 2));
+      if (n_k > 0) {
+        const int q_row = uniform(w.s.q0 + w.t0), q_b = uniform(w.s.qb), k_row = uniform(w.s.k0 + w.ta * kTile),
+                  k_b = uniform(w.s.kb);
+        const uint32_t qbar = smem_u32(&bar_q);
+        if (elect()) {
+          const uint32_t bytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
+          mbar_expect(qbar, pairs ? 2 * bytes : bytes);
+          for (int s = 0; s < (pairs ? 2 : 1); ++s)
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group, q_row + s * p.tt, q_b,
+                          qbar);
+        }
+        __syncwarp();
+        int slot = 0, issued = 0;
+        unsigned phase = 0;
+        const auto load = [&](const CUtensorMap *map, int j) {
+          if (!warp_wait(smem_u32(&bar_empty[slot]), phase ^ 1u, &gave_up)) return false;
+          if (elect()) {
+            const uint32_t fb = smem_u32(&bar_full[slot]);
+            mbar_expect(fb, C::kSlotBytes);
+#pragma unroll
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, map, h * 64, k_row + j * kTile, kvh, k_b, fb);
           }
-          const uint32_t fb = smem_u32(&bar_full[slot]);
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(fb), "r"(C::kSlotBytes) : "memory");
-          const int row = w.s.k0 + (w.ta + j) * kTile;
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, is_v ? &map_v : &map_k, h * 64, row, kvh, w.s.kb, fb);
-          issued = pos + 1;
+          __syncwarp();
+          if (++slot == C::kSlots) slot = 0, phase ^= 1u;
+          ++issued;
+          return true;
+        };
+        if (pairs) {
+          for (int j = 0; j < n_k; ++j)
+            if (!load(&map_k, j) || !load(&map_v, j)) break;
+        } else if (load(&map_k, 0)) {
+          for (int j = 0; j < n_k; ++j)
+            if ((j + 1 < n_k && !load(&map_k, j + 1)) || !load(&map_v, j)) break;
         }
         // copies in flight land before the CTA can end (bounded)
-        (void)mbar_wait(qbar, 0, &gave_up);
+        (void)warp_wait(qbar, 0, &gave_up);
         for (int pos = max(0, issued - C::kSlots); pos < issued; ++pos)
-          for (unsigned k = 0; k < kWaitLimit; ++k) {
-            if (mbar_try(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u)) break;
+          for (unsigned i = 0; i < kWaitLimit; ++i) {
+            if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar_full[pos % C::kSlots]),
+                                                 static_cast<unsigned>(pos / C::kSlots) & 1u)))
+              break;
             __nanosleep(32);
           }
       }
     } else if (warp == 9) {
-      if (lane == 0 && nk > 0) {
+      if (n_k > 0) {
         constexpr uint32_t id_s = idesc_bf16(kTile, 0), id_o = idesc_bf16(HDP, 1);
-        unsigned clean_ph = 0, p_ph[2] = {0, 0};
-        bool o_open[2] = {false, false};  // has the stream's O been written?
-        bool ok = mbar_wait(smem_u32(&bar_q), 0, &gave_up);
-        const auto wait_full = [&](int pos) {
-          return mbar_wait(smem_u32(&bar_full[pos % C::kSlots]), static_cast<unsigned>(pos / C::kSlots) & 1u, &gave_up);
+        const uint32_t dq = desc_kmajor(smem_q), dk = desc_kmajor(ring), dv = desc_mnmajor(ring);
+        constexpr uint32_t kSlotStep = C::kSlotBytes >> 4;
+        unsigned clean_ph = 0, p_ph0 = 0, p_ph1 = 0, open0 = 0, open1 = 0;  // open: the stream's O has been written
+        int slot = 0;
+        unsigned phase = 0;
+        bool ok = warp_wait(smem_u32(&bar_q), 0, &gave_up);
+        // K and V tiles are taken in ring order: waits for the next one, returns its slot
+        const auto next = [&](int &taken) {
+          taken = slot;
+          const bool r = warp_wait(smem_u32(&bar_full[slot]), phase, &gave_up);
+          if (++slot == C::kSlots) slot = 0, phase ^= 1u;
+          return r;
         };
-        const auto scores = [&](int s, int pos) {  // S of stream s from the K tile at ring position pos
-          const uint32_t q = smem_q + (pair ? s : 0) * C::kSlotBytes, k = ring + (pos % C::kSlots) * C::kSlotBytes;
+        // S of stream s from the K tile in slot k; `last`: nothing else reads that tile
+        const auto scores = [&](int s, uint32_t q, int k, bool last) {
+          fence_after();
+          if (elect()) {
+            const uint32_t a = dq + q, b = dk + k * kSlotStep;
 #pragma unroll
-          for (int i = 0; i < C::kHalves * 4; ++i) {
-            const uint32_t o = (i / 4) * 16384 + (i % 4) * 32;
-            mma_ss(tmem_s[s], desc_kmajor(q + o), desc_kmajor(k + o), id_s, i > 0);
+            for (int i = 0; i < C::kHalves * 4; ++i)
+              mma_ss(s * 128, a + (i / 4) * 1024 + (i % 4) * 2, b + (i / 4) * 1024 + (i % 4) * 2, id_s, i > 0);
+            mma_commit(smem_u32(&bar_s[s]));
+            if (last) mma_commit(smem_u32(&bar_empty[k]));
           }
-          mma_commit(smem_u32(&bar_s[s]));
+          __syncwarp();
         };
-        const auto values = [&](int s, int pos) {  // O of stream s from its P and the V tile at pos
-          const uint32_t v = ring + (pos % C::kSlots) * C::kSlotBytes;
+        // O of stream s from its P and the V tile in slot v; `end`: the stream's last
+        const auto values = [&](int s, int v, unsigned &open, bool last, bool end) {
+          fence_after();
+          if (elect()) {
+            const uint32_t b = dv + v * kSlotStep;
+            mma_ts(256 + s * 128, s * 128, b, id_o, open);
 #pragma unroll
-          for (int i = 0; i < kTile / 16; ++i)
-            mma_ts(tmem_o[s], tmem_s[s] + i * 8, desc_mnmajor(v + i * 2048), id_o, (i > 0 || o_open[s]) ? 1u : 0u);
-          o_open[s] = true;
+            for (int i = 1; i < kTile / 16; ++i) mma_ts(256 + s * 128, s * 128 + i * 8, b + i * 128, id_o, 1);
+            if (last) mma_commit(smem_u32(&bar_empty[v]));
+            if (end) mma_commit(smem_u32(&bar_o[s]));
+          }
+          __syncwarp();
+          open = 1;
         };
         // V tile j has landed; warps 10-11 look it over (while the softmax runs) where some row does not see all of it
-        const auto wait_v = [&](int j, int pos) {
-          if (!wait_full(pos)) return false;
-          if (j >= first_masked) mbar_arrive(smem_u32(&bar_dirty));
+        const auto wait_v = [&](int j, int &v) {
+          if (!next(v)) return false;
+          if (j >= n_full && elect()) mbar_arrive(smem_u32(&bar_dirty));
+          __syncwarp();
           return true;
         };
         const auto wait_clean = [&](int j) {
-          if (j < first_masked) return true;
-          const bool r = mbar_wait(smem_u32(&bar_clean), clean_ph, &gave_up);
+          if (j < n_full) return true;
+          const bool r = warp_wait(smem_u32(&bar_clean), clean_ph, &gave_up);
           clean_ph ^= 1u;
           return r;
         };
-        const auto wait_p = [&](int s) {
-          const bool r = mbar_wait(smem_u32(&bar_p[s]), p_ph[s], &gave_up);
-          p_ph[s] ^= 1u;
+        const auto wait_p = [&](int s, unsigned &ph) {
+          const bool r = warp_wait(smem_u32(&bar_p[s]), ph, &gave_up);
+          ph ^= 1u;
           return r;
         };
-        const auto release = [&](int pos) { mma_commit(smem_u32(&bar_empty[pos % C::kSlots])); };
-        if (ok && pair) {
-          ok = wait_full(0);
-          fence_after();
+        int k = 0, v = 0;
+        if (ok && pairs) {
+          constexpr uint32_t kSecond = kSlotStep;  // the second Q tile
+          ok = next(k);
           if (ok) {
-            if (n0 > 0) scores(0, 0);
-            scores(1, 0);
-            release(0);
+            if (n_0 > 0) scores(0, 0, k, false);
+            scores(1, kSecond, k, true);
           }
-          for (int j = 0; ok && j < nk; ++j) {
-            const int pv = pos_v(j), pk = pos_k(j + 1);
-            if (!(ok = wait_v(j, pv))) break;
-            const bool more = j + 1 < nk;
-            if (j < n0 && !(ok = wait_p(0))) break;
+          for (int j = 0; ok && j < n_k; ++j) {
+            if (!(ok = wait_v(j, v))) break;
+            const bool more = j + 1 < n_k;
+            if (j < n_0 && !(ok = wait_p(0, p_ph0))) break;
             if (!(ok = wait_clean(j))) break;
-            if (j < n0) {
-              fence_after();
-              values(0, pv);
-              if (j + 1 == n0) mma_commit(smem_u32(&bar_o[0]));
-            }
+            if (j < n_0) values(0, v, open0, false, j + 1 == n_0);
             if (more) {
-              if (!(ok = wait_full(pk))) break;
-              fence_after();
-              if (j + 1 < n0) scores(0, pk);
+              if (!(ok = next(k))) break;
+              if (j + 1 < n_0) scores(0, 0, k, false);
             }
-            if (!(ok = wait_p(1))) break;
-            fence_after();
-            values(1, pv);
-            release(pv);
-            if (more) {
-              scores(1, pk);
-              release(pk);
-            } else {
-              mma_commit(smem_u32(&bar_o[1]));
-            }
+            if (!(ok = wait_p(1, p_ph1))) break;
+            values(1, v, open1, true, !more);
+            if (more) scores(1, kSecond, k, true);
           }
         } else if (ok) {
-          ok = wait_full(0);
-          fence_after();
-          if (ok) {
-            scores(0, 0);
-            release(0);
-          }
-          for (int j = 0; ok && j < nk; ++j) {
-            const int s = j & 1;
-            if (j + 1 < nk) {
-              const int pk = pos_k(j + 1);
-              if (!(ok = wait_full(pk))) break;
-              fence_after();
-              scores(s ^ 1, pk);
-              release(pk);
+          // solo: key tile j belongs to stream j mod 2
+          const auto step = [&](int j, int s, unsigned &ph, unsigned &open) {
+            if (j + 1 < n_k) {
+              if (!next(k)) return false;
+              scores(s ^ 1, 0, k, true);
             }
-            const int pv = pos_v(j);
-            if (!(ok = wait_v(j, pv)) || !(ok = wait_p(s)) || !(ok = wait_clean(j))) break;
-            fence_after();
-            values(s, pv);
-            release(pv);
-            if (j + 2 >= nk) mma_commit(smem_u32(&bar_o[s]));
+            if (!wait_v(j, v) || !wait_p(s, ph) || !wait_clean(j)) return false;
+            values(s, v, open, true, j + 2 >= n_k);
+            return true;
+          };
+          ok = next(k);
+          if (ok) scores(0, 0, k, true);
+          for (int j = 0; ok && j < n_k; j += 2) {
+            ok = step(j, 0, p_ph0, open0);
+            if (ok && j + 1 < n_k) ok = step(j + 1, 1, p_ph1, open1);
           }
         }
         // nothing of this CTA is in flight in the tensor core when it ends
-        mma_commit(smem_u32(&bar_drain));
-        for (unsigned k = 0; k < kWaitLimit && !mbar_try(smem_u32(&bar_drain), 0); ++k) __nanosleep(32);
+        if (elect()) mma_commit(smem_u32(&bar_drain));
+        __syncwarp();
+        for (unsigned i = 0; i < kWaitLimit; ++i) {
+          if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar_drain), 0))) break;
+          __nanosleep(32);
+        }
       }
     } else {
       // ---- V tiles that some row does not see in full: what is not finite becomes zero
@@ -745,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(smem_u32(&bar_clean));
       }
     }
-  } else {
+  } else if (w.live) {  // uniform over the CTA
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax: one thread per row of the stream's tile
     const int s = warp >> 2;
@@ -758,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tok = min(row / p.group, cnt - 1);
     const int tok0 = wrow / p.group, tok1 = min((wrow + 31) / p.group, cnt - 1);
     const uint32_t lanes = static_cast<uint32_t>(wrow) << 16;
-    const uint32_t ts = tmem_s[s] + lanes, to = tmem_o[s] + lanes;
+    const uint32_t ts = s * 128 + lanes, to = 256 + s * 128 + lanes;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
     const int mine = pair ? (s ? nk : n0) : (nk + 1 - s) / 2;
@@ -781,11 +859,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 128; ++i)
             if (!((bits[i / 32] >> (i % 32)) & 1u)) x[i] = 0xff800000u;  // -infinity
         }
+        // a NaN among the scores makes the row's maximum, and with it the row, NaN
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) top[i % 4] = fmaxf(top[i % 4], __uint_as_float(x[i]));
-        const float mz = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
-        const bool follow = mz > m + kFollow;
+        for (int i = 0; i < 128; i += 2)
+          top[i / 2 % 4] = max_nan3(top[i / 2 % 4], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        const float mz = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * sl;
+        const bool follow = !(mz <= m + kFollow);
         if (__any_sync(0xffffffffu, follow)) {
           const float mn = follow ? mz : m;
           const float a = m == -INFINITY ? 0.f : ex2(m - mn);
@@ -804,21 +884,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= a;
           m = mn;
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // nothing seen yet: any finite reference; a score of infinity: NaN, as infinity minus itself
+        const float ref = m == -INFINITY ? 0.f : (m == INFINITY ? __uint_as_float(0x7fffffffu) : m);
+        const uint64_t sl2 = two(sl), ref2 = two(-ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float e0 = ex2(fmaf(__uint_as_float(x[32 * c + 2 * i]), sl, -ref));
-            const float e1 = ex2(fmaf(__uint_as_float(x[32 * c + 2 * i + 1]), sl, -ref));
-            sum[i % 4] += e0 + e1;
+            const uint64_t z = fma2(two(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sl2, ref2);
+            float e0, e1;
+            if (i % kPolyOf < kPoly) {
+              exp2_poly(z, e0, e1);
+            } else {
+              e0 = ex2(low_of(z));
+              e1 = ex2(high_of(z));
+            }
+            sum[i % 2] = add2(sum[i % 2], two(__float_as_uint(e0), __float_as_uint(e1)));
             pk[i] = pack_bf16(e0, e1);  // the matrix product takes BF16; the sum keeps fp32
           }
           tmem_st16(ts + 16 * c, pk);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const uint64_t both = add2(sum[0], sum[1]);
+        l += low_of(both) + high_of(both);
         tmem_wait_st();
       }
       fence_before();
@@ -843,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         join[0][row] = m;
         join[1][row] = l;
         if (active && ok && mine > 0)
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < HDP / 32; ++c) {
             uint32_t o[32];
             tmem_ld32(to + 32 * c, o);
@@ -872,7 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t token = w.s.q0 + t0 + tok;
       uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
                       static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < HDP / 32; ++c) {
         float o[32];
         if (mine > 0) {
@@ -885,7 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           if (second) o[i] = o[i] * a0 + joined[(32 * c + i) * kTile + row] * a1;
-          o[i] = l == 0.f ? 0.f : o[i] * inv;
+          o[i] *= inv;
         }
         if (!valid) continue;
         if (p.splits > 1) {
@@ -916,7 +1005,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0 && gave_up && p.status) atomicOr(p.status, AIB_STATUS_WAIT_TIMEOUT);
   if (warp == 9) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
   }
 }
 
@@ -946,28 +1035,26 @@ __global__ void __launch_bounds__(HDP * 4) attn_join_kernel(const __grid_constan
   const int64_t share = static_cast<int64_t>(p.d.nkv) * p.tpi * (kTile * (HDP + 2));
   const float *part = p.d.workspace + (static_cast<int64_t>(item) * p.splits * p.d.nkv * p.tpi + kvh * p.tpi + tile) *
                                           (kTile * (HDP + 2));
-  for (int sp = warp; sp < p.splits; sp += HDP / 8) {
+  // shares that the item's key tiles do not reach are not read; every other CTA wrote its rows in full
+  for (int sp = warp; sp < w.shares; sp += HDP / 8) {
     weight[sp][lane] = valid ? part[sp * share + HDP * kTile + row] : -INFINITY;
     sums[sp][lane] = valid ? part[sp * share + (HDP + 1) * kTile + row] : 0.f;
   }
   __syncthreads();
-  float m = -INFINITY;
-  for (int sp = 0; sp < p.splits; ++sp) m = fmaxf(m, weight[sp][lane]);
-  const float ref = m == -INFINITY ? 0.f : m;
   const int c0 = warp * 8;
-  float l = 0.f, o[8] = {};
-#pragma unroll 4
-  for (int sp = 0; sp < p.splits; ++sp) {
-    const float ls = sums[sp][lane];
-    // a share that the row's keys do not reach has a sum of zero and no O
-    const bool some = ls != 0.f && c0 < p.d.hd;
-    const float a = some ? ex2(weight[sp][lane] - ref) : 0.f;
-    l += a * ls;
-    const float *q = part + sp * share + c0 * kTile + row;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] += a * (some ? q[i * kTile] : 0.f);
-  }
   if (!valid || c0 >= p.d.hd) return;
+  float m = -INFINITY;
+  for (int sp = 0; sp < w.shares; ++sp) m = fmaxf(m, weight[sp][lane]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[8] = {};
+  const float *q = part + c0 * kTile + row;
+#pragma unroll 4
+  for (int sp = 0; sp < w.shares; ++sp) {
+    const float a = ex2(weight[sp][lane] - ref);
+    l += a * sums[sp][lane];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] += a * q[sp * share + i * kTile];
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] *= inv;
