@@ -473,26 +473,6 @@ __device__ __forceinline__ float max_nan3(float a, float b, float c) {
   return d;
 }
 
-// 2^t for two t <= 8 on the multiply-add pipe, beside the exponential unit
-// (16 results a clock and SM, which 128 x 128 weights would keep busy as long
-// as the tensor core takes for a tile). t = r + f with r the nearest integer
-// (the sum with 1.5 2^23 leaves it in the low mantissa bits) and |f| <= 1/2;
-// 2^f by the cubic 1 + f (c1 + f (c2 + f c3)) of least relative error on that
-// interval (fitted as a linear program; 1.0e-4, a fortieth of the BF16 step
-// that P is rounded to); r goes into the exponent. t is held at -127, where the cubic is
-// 1 and the exponent comes to nothing: masked scores give 0 exactly.
-__device__ __forceinline__ void exp2_poly(uint64_t t, float &e0, float &e1) {
-  t = two(__float_as_uint(fmaxf(low_of(t), -127.f)), __float_as_uint(fmaxf(high_of(t), -127.f)));
-  const uint64_t r = add2(t, two(12582912.f));
-  const uint64_t f = fma2(add2(r, two(-12582912.f)), two(-1.f), t);
-  uint64_t y = fma2(two(0.055009059607982635f), f, two(0.2422109693288803f));
-  y = fma2(y, f, two(0.6932829022407532f));
-  y = fma2(y, f, two(1.f));
-  e0 = __uint_as_float((static_cast<uint32_t>(r) << 23) + static_cast<uint32_t>(y));
-  e1 = __uint_as_float((static_cast<uint32_t>(r >> 32) << 23) + static_cast<uint32_t>(y >> 32));
-}
-// of every kPolyOf pairs of weights, kPoly take the polynomial
-constexpr int kPoly = 0, kPolyOf = 8;
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 
 // bits of the seen keys among the four 32-key words of key tile t, for this
@@ -569,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<HDP>;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bar_full[kMaxSlots], bar_empty[kMaxSlots];
-  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2], bar_o[2], bar_drain, bar_dirty, bar_clean;
+  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2][2], bar_o[2], bar_drain, bar_dirty, bar_clean;
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up, bad_seen;
   __shared__ float join[2][kTile];  // maximum and sum of stream 1's rows
@@ -589,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(smem_u32(&bar_q), 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&bar_s[s]), 1);
-      mbar_init(smem_u32(&bar_p[s]), 4);
+      mbar_init(smem_u32(&bar_p[s][0]), 4);
+      mbar_init(smem_u32(&bar_p[s][1]), 4);
       mbar_init(smem_u32(&bar_o[s]), 1);
     }
     mbar_init(smem_u32(&bar_drain), 1);
@@ -710,19 +691,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
-        // O of stream s from its P and the V tile in slot v; `end`: the stream's last
-        const auto values = [&](int s, int v, unsigned &open, bool last, bool end) {
+        // O of stream s from its P and the V tile in slot v, 64 keys and then the other 64, whose weights may still
+        // be on their way; `end`: the stream's last
+        const auto values = [&](int s, int v, unsigned &open, unsigned &ph, bool last, bool end) {
           fence_after();
+          const uint32_t b = dv + v * kSlotStep;
           if (elect()) {
-            const uint32_t b = dv + v * kSlotStep;
             mma_ts(256 + s * 128, s * 128, b, id_o, open);
 #pragma unroll
-            for (int i = 1; i < kTile / 16; ++i) mma_ts(256 + s * 128, s * 128 + i * 8, b + i * 128, id_o, 1);
+            for (int i = 1; i < kTile / 32; ++i) mma_ts(256 + s * 128, s * 128 + i * 8, b + i * 128, id_o, 1);
+          }
+          __syncwarp();
+          open = 1;
+          if (!warp_wait(smem_u32(&bar_p[s][1]), ph, &gave_up)) return false;
+          ph ^= 1u;
+          fence_after();
+          if (elect()) {
+#pragma unroll
+            for (int i = kTile / 32; i < kTile / 16; ++i)
+              mma_ts(256 + s * 128, s * 128 + i * 8, b + i * 128, id_o, 1);
             if (last) mma_commit(smem_u32(&bar_empty[v]));
             if (end) mma_commit(smem_u32(&bar_o[s]));
           }
           __syncwarp();
-          open = 1;
+          return true;
         };
         // V tile j has landed; warps 10-11 look it over (while the softmax runs) where some row does not see all of it
         const auto wait_v = [&](int j, int &v) {
@@ -737,11 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           clean_ph ^= 1u;
           return r;
         };
-        const auto wait_p = [&](int s, unsigned &ph) {
-          const bool r = warp_wait(smem_u32(&bar_p[s]), ph, &gave_up);
-          ph ^= 1u;
-          return r;
-        };
+        const auto wait_p = [&](int s, unsigned ph) { return warp_wait(smem_u32(&bar_p[s][0]), ph, &gave_up); };
         int k = 0, v = 0;
         if (ok && pairs) {
           constexpr uint32_t kSecond = kSlotStep;  // the second Q tile
@@ -755,13 +743,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool more = j + 1 < n_k;
             if (j < n_0 && !(ok = wait_p(0, p_ph0))) break;
             if (!(ok = wait_clean(j))) break;
-            if (j < n_0) values(0, v, open0, false, j + 1 == n_0);
+            if (j < n_0 && !(ok = values(0, v, open0, p_ph0, false, j + 1 == n_0))) break;
             if (more) {
               if (!(ok = next(k))) break;
               if (j + 1 < n_0) scores(0, 0, k, false);
             }
-            if (!(ok = wait_p(1, p_ph1))) break;
-            values(1, v, open1, true, !more);
+            if (!(ok = wait_p(1, p_ph1)) || !(ok = values(1, v, open1, p_ph1, true, !more))) break;
             if (more) scores(1, kSecond, k, true);
           }
         } else if (ok) {
@@ -772,8 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               scores(s ^ 1, 0, k, true);
             }
             if (!wait_v(j, v) || !wait_p(s, ph) || !wait_clean(j)) return false;
-            values(s, v, open, true, j + 2 >= n_k);
-            return true;
+            return values(s, v, open, ph, true, j + 2 >= n_k);
           };
           ok = next(k);
           if (ok) scores(0, 0, k, true);
@@ -894,25 +880,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const uint64_t z = fma2(two(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sl2, ref2);
-            float e0, e1;
-            if (i % kPolyOf < kPoly) {
-              exp2_poly(z, e0, e1);
-            } else {
-              e0 = ex2(low_of(z));
-              e1 = ex2(high_of(z));
-            }
+            const float e0 = ex2(low_of(z)), e1 = ex2(high_of(z));
             sum[i % 2] = add2(sum[i % 2], two(__float_as_uint(e0), __float_as_uint(e1)));
             pk[i] = pack_bf16(e0, e1);  // the matrix product takes BF16; the sum keeps fp32
           }
           tmem_st16(ts + 16 * c, pk);
+          if (c == 1) {  // the first 64 keys' weights can be used
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bar_p[s][0]));
+          }
         }
         const uint64_t both = add2(sum[0], sum[1]);
         l += low_of(both) + high_of(both);
         tmem_wait_st();
+      } else if (lane == 0) {
+        mbar_arrive(smem_u32(&bar_p[s][0]));
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_p[s]));
+      if (lane == 0) mbar_arrive(smem_u32(&bar_p[s][1]));
     }
     if (ok && mine > 0) ok = warp_wait(smem_u32(&bar_o[s]), 0, &gave_up);
     fence_after();
