@@ -102,8 +102,6 @@ class AttnDesc(ctypes.Structure):
         ("cu_q", P), ("cu_k", P), ("len_k", P), ("pos", P), ("mask", P),
         ("mask_batch_stride", I64), ("mask_row_stride", I64), ("mask_col_stride", I64),
         ("mask_cols", I64),
-        ("workspace", P),
-        ("workspace_floats", I64),
     ]
 
 
@@ -150,9 +148,10 @@ SIGNATURES = [
     ("aib_gemv_bf16", CI, [P, I64, P, I64, P, I64, I64, I64, CI, CI, P]),
     ("aib_gemm_bf16_tc", CI, [P, I64, P, I64, P, I64, I64, I64, I64, P, I64, P, P]),
     ("aib_gemm_bf16_tc_workspace_floats", I64, [I64, I64, I64]),
-    ("aib_attention_workspace_floats", I64, [ctypes.POINTER(AttnDesc)]),
-    ("aib_prompt_attention_bf16", CI, [ctypes.POINTER(AttnDesc), P, P]),
-    ("aib_tree_attention_bf16", CI, [ctypes.POINTER(AttnDesc), P, P]),
+    # aib_attn_desc by address: an AttnDesc or its packed bytes (runtime/seq_ops.py)
+    ("aib_attention_workspace_floats", I64, [P]),
+    ("aib_prompt_attention_bf16", CI, [P, P, I64, P, P]),
+    ("aib_tree_attention_bf16", CI, [P, P, I64, P, P]),
     ("aib_rope_cache_packed_bf16", CI, [P, I64, I64, I64, CI, CI, CI, P, P, P, P, P, ctypes.c_float, P, P, P, P, P, P,
                                         I64, P]),
     ("aib_keep_cache_rows_bf16", CI, [P, CI, I64, CI, I64, CI, P, P, P, CI, P]),

@@ -220,6 +220,7 @@ struct TcParams {
   int items;           // upper bound of the items
   float scale_log2;
   int vec_out;         // output rows allow 16-byte stores
+  float *workspace;    // shares: O, maximum and sum of their rows
   int32_t *status;
 };
 
@@ -945,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool valid = row < rows;
       const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       const int64_t unit = (static_cast<int64_t>(rest) * p.d.nkv + kvh) * p.tpi + tile;
-      float *part = p.d.workspace + unit * (kTile * (HDP + 2));
+      float *part = p.workspace + unit * (kTile * (HDP + 2));
       const int64_t token = w.s.q0 + t0 + tok;
       uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
                       static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
@@ -1021,7 +1022,7 @@ __global__ void __launch_bounds__(HDP * 4) attn_join_kernel(const __grid_constan
   const int row = quarter * 32 + lane;
   const bool valid = row < rows;
   const int64_t share = static_cast<int64_t>(p.d.nkv) * p.tpi * (kTile * (HDP + 2));
-  const float *part = p.d.workspace + (static_cast<int64_t>(item) * p.splits * p.d.nkv * p.tpi + kvh * p.tpi + tile) *
+  const float *part = p.workspace + (static_cast<int64_t>(item) * p.splits * p.d.nkv * p.tpi + kvh * p.tpi + tile) *
                                           (kTile * (HDP + 2));
   // shares that the item's key tiles do not reach are not read; every other CTA wrote its rows in full
   for (int sp = warp; sp < w.shares; sp += HDP / 8) {
@@ -1072,7 +1073,7 @@ static int check_common(const aib_attn_desc *p, const char *who) {
                           p->nkv, p->hd, kPlainMaxHd), AIB_EINVAL;
   const int64_t big = INT32_MAX - 1024;  // room for a tile behind the last row
   if (p->tokens > big || p->batch > big || p->key_rows > big)
-    return aib_set_errorf("%s: tokens, batch and key rows must be below 2^31 - 1024", who), AIB_EINVAL;
+    return aib_set_errorf("%s: tokens, batch and key rows must fit in 32 bits (below 2^31 - 1024)", who), AIB_EINVAL;
   if (!std::isfinite(p->scale)) return aib_set_errorf("%s: scale is not finite", who), AIB_EINVAL;
   return AIB_OK;
 }
@@ -1173,8 +1174,8 @@ static int sm_count() {
 }
 
 template <int HDP>
-static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, int32_t *status,
-                     cudaStream_t st) {
+static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, float *workspace,
+                     int32_t *status, cudaStream_t st) {
   // the shared-memory limit is set once per device
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
@@ -1203,6 +1204,7 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   p.scale_log2 = d.scale * 1.4426950408889634f;
   p.vec_out = aligned16(d.out) && d.out_token_stride % 8 == 0 && d.out_head_stride % 8 == 0 &&
               d.out_batch_stride % 8 == 0;
+  p.workspace = workspace;
   p.status = status;
   const int64_t grid = pl.items * pl.splits * d.nkv;
   attn_tc_kernel<HDP><<<static_cast<unsigned>(grid), kThreads, Cfg<HDP>::kSmem, st>>>(mq, mk, mv, p);
@@ -1223,15 +1225,17 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   return AIB_OK;
 }
 
-static int launch(const aib_attn_desc &d, const char *who, int32_t *status, cudaStream_t st) {
+static int launch(const aib_attn_desc &d, const char *who, float *workspace, int64_t floats, int32_t *status,
+                  cudaStream_t st) {
   const bool tree = d.mask != nullptr;
   if (tensor_cores(d, tree)) {
     const TcPlan pl = tc_plan(d, tree, sm_count());
     if (pl.items * pl.splits * d.nkv * 4 * pl.tpi > INT32_MAX) return aib_set_errorf("%s: too many rows", who), AIB_EINVAL;
     const int64_t need = tc_floats(d, pl);
-    if (need && (!d.workspace || d.workspace_floats < need))
+    if (need && (!workspace || floats < need))
       return aib_set_errorf("%s: needs a workspace of %lld floats", who, (long long)need), AIB_EINVAL;
-    return d.hd <= 64 ? launch_tc<64>(d, tree, pl, who, status, st) : launch_tc<128>(d, tree, pl, who, status, st);
+    return d.hd <= 64 ? launch_tc<64>(d, tree, pl, who, workspace, status, st)
+                      : launch_tc<128>(d, tree, pl, who, workspace, status, st);
   }
   const int64_t rows = (tree ? d.batch : 1) * d.tokens * d.nh;
   const int64_t blocks = (rows + kPlainWarps - 1) / kPlainWarps;
@@ -1246,7 +1250,8 @@ static int launch(const aib_attn_desc &d, const char *who, int32_t *status, cuda
 
 using namespace aibseq;
 
-AIB_API int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream) {
+AIB_API int aib_prompt_attention_bf16(const aib_attn_desc *desc, float *workspace, int64_t workspace_floats,
+                                      int32_t *d_status, void *stream) {
   const char *who = "prompt_attention";
   if (const int rc = check_common(desc, who)) return rc;
   aib_attn_desc p = *desc;
@@ -1255,10 +1260,11 @@ AIB_API int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *d_stat
   if (!p.q || !p.out || !p.cu_q || (p.key_rows && (!p.k || !p.v)))
     return aib_set_errorf("%s: null pointer", who), AIB_EINVAL;
   if (!p.len_k && !p.cu_k) return aib_set_errorf("%s: give cu_k (packed keys) or len_k (caches)", who), AIB_EINVAL;
-  return launch(p, who, d_status, static_cast<cudaStream_t>(stream));
+  return launch(p, who, workspace, workspace_floats, d_status, static_cast<cudaStream_t>(stream));
 }
 
-AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream) {
+AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, float *workspace, int64_t workspace_floats,
+                                    int32_t *d_status, void *stream) {
   const char *who = "tree_attention";
   if (const int rc = check_common(desc, who)) return rc;
   const aib_attn_desc &p = *desc;
@@ -1268,7 +1274,7 @@ AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *d_status
   if (p.tokens == 0 || p.batch == 0) return AIB_OK;
   if (!p.q || !p.out || !p.pos || !p.mask || (p.key_rows && (!p.k || !p.v)))
     return aib_set_errorf("%s: null pointer", who), AIB_EINVAL;
-  return launch(p, who, d_status, static_cast<cudaStream_t>(stream));
+  return launch(p, who, workspace, workspace_floats, d_status, static_cast<cudaStream_t>(stream));
 }
 
 AIB_API int64_t aib_attention_workspace_floats(const aib_attn_desc *d) {

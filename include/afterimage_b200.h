@@ -350,13 +350,11 @@ typedef struct aib_attn_desc {
   const uint8_t *mask;  /* tree: [batch, tokens, mask_cols], nonzero where the query sees the drafted column */
   int64_t mask_batch_stride, mask_row_stride, mask_col_stride;
   int64_t mask_cols;    /* tree: drafted tokens in the cache, at slots pos .. pos + mask_cols - 1 */
-  float *workspace;     /* aib_attention_workspace_floats(desc) floats (NULL when 0); each call in flight
-                           needs its own */
-  int64_t workspace_floats;
 } aib_attn_desc;
 
-/* Floats of workspace the descriptor's call needs (0: none). The pointers
- * need not be set except for their being NULL or not. */
+/* Floats of workspace the descriptor's call needs on the current device (0:
+ * none). Each call in flight needs its own; nothing in it needs to start at
+ * zero. */
 int64_t aib_attention_workspace_floats(const aib_attn_desc *desc);
 /* Causal attention of packed prompts: sequence b has the query rows
  * cu_q[b] .. cu_q[b + 1] - 1 (m of them) and L keys; its row i sees the keys
@@ -364,11 +362,13 @@ int64_t aib_attention_workspace_floats(const aib_attn_desc *desc);
  * that see nothing are zero; rows outside every sequence are not written.
  * Offsets are cut to the tensors' extents. d_status (optional): a bounded
  * wait that gives up sets AIB_STATUS_WAIT_TIMEOUT. */
-int aib_prompt_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream);
+int aib_prompt_attention_bf16(const aib_attn_desc *desc, float *workspace, int64_t workspace_floats, int32_t *d_status,
+                              void *stream);
 /* Attention of drafted tokens over caches: every query of sequence b sees
  * the slots before pos[b], and slot pos[b] + j where mask[b, i, j]. Slots
  * outside [0, key_rows) are not seen. */
-int aib_tree_attention_bf16(const aib_attn_desc *desc, int32_t *d_status, void *stream);
+int aib_tree_attention_bf16(const aib_attn_desc *desc, float *workspace, int64_t workspace_floats, int32_t *d_status,
+                            void *stream);
 /* qkv [n, (nh + 2 nkv) * hd] with row stride qkv_stride; row cu[b] + i is
  * token i of sequence b. RMSNorm of q and k over hd (when both weights are
  * given), rotary embedding at place start[b] + depth[row] (depth NULL: i),

@@ -171,24 +171,24 @@ def _desc(**kw):
 def test_attention_c_entries_refuse(entry, kw, text):
     L = _lib.load()
     d = _desc(**kw)
-    assert getattr(L, entry)(d, None, None) == _lib.AIB_EINVAL
+    assert getattr(L, entry)(ctypes.byref(d), None, 0, None, None) == _lib.AIB_EINVAL
     assert text in L.aib_last_error()
 
 
 def test_attention_c_entries_refuse_what_only_one_takes():
     L = _lib.load()
-    assert L.aib_prompt_attention_bf16(None, None, None) == _lib.AIB_EINVAL
-    assert L.aib_prompt_attention_bf16(_desc(cu_q=None), None, None) == _lib.AIB_EINVAL
-    assert L.aib_prompt_attention_bf16(_desc(cu_k=None), None, None) == _lib.AIB_EINVAL
+    assert L.aib_prompt_attention_bf16(None, None, 0, None, None) == _lib.AIB_EINVAL
+    assert L.aib_prompt_attention_bf16(ctypes.byref(_desc(cu_q=None)), None, 0, None, None) == _lib.AIB_EINVAL
+    assert L.aib_prompt_attention_bf16(ctypes.byref(_desc(cu_k=None)), None, 0, None, None) == _lib.AIB_EINVAL
     assert b"cu_k" in L.aib_last_error()
-    assert L.aib_tree_attention_bf16(_desc(pos=None), None, None) == _lib.AIB_EINVAL
-    assert L.aib_tree_attention_bf16(_desc(mask=None), None, None) == _lib.AIB_EINVAL
-    assert L.aib_tree_attention_bf16(_desc(mask_cols=9), None, None) == _lib.AIB_EINVAL
+    assert L.aib_tree_attention_bf16(ctypes.byref(_desc(pos=None)), None, 0, None, None) == _lib.AIB_EINVAL
+    assert L.aib_tree_attention_bf16(ctypes.byref(_desc(mask=None)), None, 0, None, None) == _lib.AIB_EINVAL
+    assert L.aib_tree_attention_bf16(ctypes.byref(_desc(mask_cols=9)), None, 0, None, None) == _lib.AIB_EINVAL
     assert b"columns" in L.aib_last_error()
     # nothing to do: no CUDA call
     for kw in (dict(tokens=0), dict(batch=0)):
-        assert L.aib_prompt_attention_bf16(_desc(**kw), None, None) == _lib.AIB_OK
-        assert L.aib_tree_attention_bf16(_desc(**kw), None, None) == _lib.AIB_OK
+        assert L.aib_prompt_attention_bf16(ctypes.byref(_desc(**kw)), None, 0, None, None) == _lib.AIB_OK
+        assert L.aib_tree_attention_bf16(ctypes.byref(_desc(**kw)), None, 0, None, None) == _lib.AIB_OK
 
 
 def test_cache_c_entries_refuse():
