@@ -236,7 +236,19 @@ struct Item {
   bool live;
 };
 
-__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+// Items of sequence i (`unit` tokens each).
+__device__ __forceinline__ int items_of(const TcParams &p, int i) {
+  const int unit = p.tt * p.tpi;
+  const int q0 = cut(p.d.cu_q[i], 0, p.d.tokens);
+  return (cut(p.d.cu_q[i + 1], q0, p.d.tokens) - q0 + unit - 1) / unit;
+}
+// F(l) of find_item. Collective over the warp.
+__device__ __forceinline__ int items_at_or_above(const TcParams &p, int l) {
+  int f = 0;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < static_cast<int>(p.d.batch); i += 32) f += max(0, items_of(p, i) - l);
+  return __reduce_add_sync(0xffffffffu, f);
+}
 
 // Item number -> sequence and first tile. Prompts: items are numbered from
 // the last tiles of the longest prompts down (they see the most keys; the
@@ -244,50 +256,44 @@ __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffff
 // in sequence b, the items at level l (the l-th of their sequence) or above
 // are F(l) = sum_b max(0, P_b - l); a binary search finds the item's level.
 // Collective over the warp.
-__device__ __forceinline__ bool find_item(const TcParams &p, int item, int &b, int &level) {
-  const int unit = p.tt * p.tpi;
-  const int batch = static_cast<int>(p.d.batch), tokens = static_cast<int>(p.d.tokens);
-  if (p.d.mask) {
-    const int per = (tokens + unit - 1) / unit;
-    b = item / per;
-    level = item - b * per;
-    return b < batch;
-  }
-  const int lane = threadIdx.x & 31;
-  const auto items_of = [&](int i) {
-    const int q0 = cut(p.d.cu_q[i], 0, tokens);
-    return (cut(p.d.cu_q[i + 1], q0, tokens) - q0 + unit - 1) / unit;
-  };
-  if (batch == 1) {
-    b = 0;
-    level = items_of(0) - 1 - item;
-    return level >= 0;
-  }
-  const int first = lane < batch ? items_of(lane) : 0;  // the common case needs no second read
-  const auto at_or_above = [&](int l) {
-    int f = max(0, first - l);
-    for (int i = lane + 32; i < batch; i += 32) f += max(0, items_of(i) - l);
-    return warp_sum(f);
-  };
-  if (at_or_above(0) <= item) return false;
-  int lo = 0, hi = (tokens + unit - 1) / unit;  // F(lo) > item >= F(hi)
+__device__ __forceinline__ bool find_among_prompts(const TcParams &p, int item, int &b, int &level) {
+  const int lane = threadIdx.x & 31, batch = static_cast<int>(p.d.batch);
+  if (items_at_or_above(p, 0) <= item) return false;
+  int lo = 0, hi = static_cast<int>(p.d.tokens);  // F(lo) > item >= F(hi)
+#pragma unroll 1
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (at_or_above(mid) > item) lo = mid; else hi = mid;
+    const int mid = lo + (hi - lo) / 2;
+    if (items_at_or_above(p, mid) > item) lo = mid; else hi = mid;
   }
-  int rank = item - at_or_above(lo + 1);  // among the sequences that reach this level
+  int rank = item - items_at_or_above(p, lo + 1);  // among the sequences that reach this level
+  level = lo;
+#pragma unroll 1
   for (int i0 = 0; i0 < batch; i0 += 32) {
-    const int i = i0 + lane;
-    unsigned has = __ballot_sync(0xffffffffu, i < batch && (i0 == 0 ? first : items_of(i)) > lo);
+    unsigned has = __ballot_sync(0xffffffffu, i0 + lane < batch && items_of(p, i0 + lane) > lo);
     if (rank < __popc(has)) {
+#pragma unroll 1
       for (; rank > 0; --rank) has &= has - 1;
       b = i0 + __ffs(has) - 1;
-      level = lo;
       return true;
     }
     rank -= __popc(has);
   }
   return false;
+}
+__device__ __forceinline__ bool find_item(const TcParams &p, int item, int &b, int &level) {
+  if (p.d.mask) {
+    const int unit = p.tt * p.tpi, tokens = static_cast<int>(p.d.tokens);
+    const int per = tokens <= unit ? 1 : (tokens + unit - 1) / unit;
+    b = per == 1 ? item : item / per;
+    level = item - b * per;
+    return b < static_cast<int>(p.d.batch);
+  }
+  if (p.d.batch == 1) {
+    b = 0;
+    level = items_of(p, 0) - 1 - item;
+    return level >= 0;
+  }
+  return find_among_prompts(p, item, b, level);
 }
 
 __device__ __forceinline__ void make_tile(const TcParams &p, const Seq &s, int t, bool used, int &cnt, int &end,
@@ -308,7 +314,7 @@ __device__ __forceinline__ Item make_item(const TcParams &p, int item, int split
   make_tile(p, w.s, w.t0, true, w.cnt0, w.end0, w.low0);
   make_tile(p, w.s, w.t0 + p.tt, p.tpi > 1, w.cnt1, w.end1, w.low1);
   const int tiles = (max(w.end0, w.end1) + kTile - 1) / kTile;
-  const int per = (tiles + p.splits - 1) / p.splits;
+  const int per = p.splits == 1 ? tiles : (tiles + p.splits - 1) / p.splits;
   w.shares = per ? (tiles + per - 1) / per : 0;
   w.ta = min(tiles, split * per);
   w.tb = min(tiles, w.ta + per);
@@ -341,6 +347,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, unsigned parity) {
 // matrix and copy instructions (their operands are uniform registers) is
 // faster for.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, unsigned parity, volatile int *gave_up) {
+#pragma unroll 1
   for (unsigned n = 0; n < kWaitLimit; ++n) {
     if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
     if (n > 256) {
@@ -416,6 +423,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *v) {
       : AIB_R8(v, 0), AIB_R8(v, 8), AIB_R8(v, 16), AIB_R8(v, 24)
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : AIB_R8(v, 0), AIB_R8(v, 8)
+      : "r"(addr));
+}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
@@ -429,6 +442,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
           addr),
       AIB_I8(v, 0), AIB_I8(v, 8)
       : "memory");
+}
+__device__ __forceinline__ float tmem_ld1(uint32_t addr) {
+  float v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void tmem_st1(uint32_t addr, float v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -495,6 +516,7 @@ __device__ __forceinline__ void seen_words(const TcParams &p, const Seq &s, int 
   const uint8_t *m = p.d.mask + static_cast<int64_t>(s.qb) * p.d.mask_batch_stride;
 #pragma unroll
   for (int c = 0; c < 4; ++c) bits[c] = 0;
+#pragma unroll 1
   for (int a = warp_tok0; a <= warp_tok1; ++a) {
     const uint8_t *row = m + static_cast<int64_t>(t0 + a) * p.d.mask_row_stride;
 #pragma unroll
@@ -519,10 +541,8 @@ __device__ __forceinline__ void add_not_finite(const TcParams &p, const Seq &s, 
   const uint16_t *v = static_cast<const uint16_t *>(p.d.v) + s.kb * p.d.v_batch_stride + s.k0 * p.d.v_token_stride +
                       kvh * p.d.v_head_stride;
 #pragma unroll 1
-  for (int c0 = 0; c0 < HDP; c0 += 32) {
-    uint32_t o[32];
-    tmem_ld32(to + c0, o);
-    tmem_wait_ld();
+  for (int c = 0; c < p.d.hd; ++c) {
+    float o = tmem_ld1(to + c);
 #pragma unroll 1
     for (int t = first; t < last; t += step) {
       uint32_t bits[4];
@@ -532,13 +552,11 @@ __device__ __forceinline__ void add_not_finite(const TcParams &p, const Seq &s, 
         const int key = t * kTile + i;
         const uint32_t word = i < 64 ? (i < 32 ? bits[0] : bits[1]) : (i < 96 ? bits[2] : bits[3]);
         if (key >= s.L || !((word >> (i & 31)) & 1u)) continue;
-        const uint16_t *vr = v + key * p.d.v_token_stride + c0;
-#pragma unroll
-        for (int d = 0; d < 32; ++d)
-          if (c0 + d < p.d.hd && not_finite_bf16(vr[d])) o[d] = __float_as_uint(__uint_as_float(o[d]) + b2f(vr[d]));
+        const uint16_t x = v[key * p.d.v_token_stride + c];
+        if (not_finite_bf16(x)) o += b2f(x);
       }
     }
-    tmem_st32(to + c0, o);
+    tmem_st1(to + c, o);
   }
   tmem_wait_st();
 }
@@ -553,16 +571,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2][2], bar_o[2], bar_drain, bar_dirty, bar_clean;
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up, bad_seen;
-  __shared__ float join[2][kTile];  // maximum and sum of stream 1's rows
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int kvh = blockIdx.x % p.d.nkv;
-  const int rest = blockIdx.x / p.d.nkv;
-  const int split = rest % p.splits;
+  // (all kv heads of the largest item first: with the items of one head after the other the mixed prompts took a
+  // sixth longer)
+  const int item = blockIdx.x / p.d.nkv, kvh = blockIdx.x - item * p.d.nkv, split = blockIdx.y;
   const uint32_t smem_q = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = smem_q + 2 * C::kSlotBytes;
 
-  if (threadIdx.x == 0) {
+  if (warp == 8 && elect()) {
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(smem_u32(&bar_full[i]), 1);
       mbar_init(smem_u32(&bar_empty[i]), 1);
@@ -580,8 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     gave_up = 0;
     bad_seen = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 8 && lane == 0) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
@@ -592,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
   }
-  const Item w = make_item(p, rest / p.splits, split);
+  const Item w = make_item(p, item, split);
 
   const bool pair = w.live && w.cnt1 > 0;
   // pair: key tiles of each stream (the second tile's tokens are later: they see as many or more);
@@ -603,14 +619,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int first_masked = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
 
   const int pairs = uniform(pair), n_k = uniform(nk), n_0 = uniform(n0), n_full = uniform(first_masked);
+  // The ring holds the tiles in the order in which the matrix instructions want them: K0 V0 K1 V1 ... for a pair,
+  // K0 K1 V0 K2 V1 ... solo.
+  const auto pos_v = [&](int j) { return pairs ? 2 * j + 1 : (j == n_k - 1 ? 2 * n_k - 1 : 2 * j + 2); };
+  const auto at = [&](int pos, int &j) {  // what is at a ring position: tile number, and whether it is V's
+    const bool end = pos == 2 * n_k - 1, odd = pos & 1;
+    const bool is_v = pairs ? odd : (pos > 0 && (!odd || end));
+    j = pairs ? pos >> 1 : (end ? n_k - 1 : (is_v ? pos / 2 - 1 : (pos + 1) / 2));
+    return is_v;
+  };
+  const int early = min(2 * n_k, C::kSlots);  // tiles that fit the empty ring: asked for before anything else
+  const int k_row = uniform(w.s.k0 + w.ta * kTile), k_b = uniform(w.s.kb);
+  const auto fetch = [&](const CUtensorMap *map, int j, int slot) {
+    if (elect()) {
+      const uint32_t fb = smem_u32(&bar_full[slot]);
+      mbar_expect(fb, C::kSlotBytes);
+#pragma unroll
+      for (int h = 0; h < C::kHalves; ++h)
+        tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, map, h * 64, k_row + j * kTile, kvh, k_b, fb);
+    }
+    __syncwarp();
+  };
+  if (warp == 8 && n_k > 0) {
+    const int q_row = uniform(w.s.q0 + w.t0), q_b = uniform(w.s.qb);
+    if (elect()) {
+      const uint32_t qbar = smem_u32(&bar_q);
+      const uint32_t bytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
+      mbar_expect(qbar, pairs ? 2 * bytes : bytes);
+      for (int s = 0; s < (pairs ? 2 : 1); ++s)
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group, q_row + s * p.tt, q_b,
+                      qbar);
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int pos = 0; pos < early; ++pos) {
+      int j;
+      const bool is_v = at(pos, j);
+      fetch(is_v ? &map_v : &map_k, j, pos);
+    }
+  }
   __syncthreads();
   fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the whole tensor memory is taken, so it starts at column 0: S (and P) of stream s at 128 s, O at 256 + 128 s
-
-  // The ring holds the tiles in the order in which the matrix instructions want them: K0 V0 K1 V1 ... for a pair,
-  // K0 K1 V0 K2 V1 ... solo.
-  const auto pos_v = [&](int j) { return pair ? 2 * j + 1 : (j == nk - 1 ? 2 * nk - 1 : 2 * j + 2); };
 
   // 384 threads start with 168 registers each; the softmax warps take over what the others leave
   // (256 x 216 + 128 x 72 = 384 x 168)
@@ -618,44 +670,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
       if (n_k > 0) {
-        const int q_row = uniform(w.s.q0 + w.t0), q_b = uniform(w.s.qb), k_row = uniform(w.s.k0 + w.ta * kTile),
-                  k_b = uniform(w.s.kb);
-        const uint32_t qbar = smem_u32(&bar_q);
-        if (elect()) {
-          const uint32_t bytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
-          mbar_expect(qbar, pairs ? 2 * bytes : bytes);
-          for (int s = 0; s < (pairs ? 2 : 1); ++s)
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_4d(smem_q + s * C::kSlotBytes + h * 16384, &map_q, h * 64, kvh * p.group, q_row + s * p.tt, q_b,
-                          qbar);
-        }
-        __syncwarp();
-        int slot = 0, issued = 0;
-        unsigned phase = 0;
-        const auto load = [&](const CUtensorMap *map, int j) {
-          if (!warp_wait(smem_u32(&bar_empty[slot]), phase ^ 1u, &gave_up)) return false;
-          if (elect()) {
-            const uint32_t fb = smem_u32(&bar_full[slot]);
-            mbar_expect(fb, C::kSlotBytes);
-#pragma unroll
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_4d(ring + slot * C::kSlotBytes + h * 16384, map, h * 64, k_row + j * kTile, kvh, k_b, fb);
-          }
-          __syncwarp();
+        int slot = 0, issued = early;
+        unsigned phase = 0;  // of the slot's release that the next load waits for
+#pragma unroll 1
+        for (; issued < 2 * n_k; ++issued) {
+          int j;
+          const bool is_v = at(issued, j);
+          if (!warp_wait(smem_u32(&bar_empty[slot]), phase, &gave_up)) break;
+          fetch(is_v ? &map_v : &map_k, j, slot);
           if (++slot == C::kSlots) slot = 0, phase ^= 1u;
-          ++issued;
-          return true;
-        };
-        if (pairs) {
-          for (int j = 0; j < n_k; ++j)
-            if (!load(&map_k, j) || !load(&map_v, j)) break;
-        } else if (load(&map_k, 0)) {
-          for (int j = 0; j < n_k; ++j)
-            if ((j + 1 < n_k && !load(&map_k, j + 1)) || !load(&map_v, j)) break;
         }
         // copies in flight land before the CTA can end (bounded)
-        (void)warp_wait(qbar, 0, &gave_up);
+        (void)warp_wait(smem_u32(&bar_q), 0, &gave_up);
+#pragma unroll 1
         for (int pos = max(0, issued - C::kSlots); pos < issued; ++pos)
+#pragma unroll 1
           for (unsigned i = 0; i < kWaitLimit; ++i) {
             if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar_full[pos % C::kSlots]),
                                                  static_cast<unsigned>(pos / C::kSlots) & 1u)))
@@ -668,8 +697,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t id_s = idesc_bf16(kTile, 0), id_o = idesc_bf16(HDP, 1);
         const uint32_t dq = desc_kmajor(smem_q), dk = desc_kmajor(ring), dv = desc_mnmajor(ring);
         constexpr uint32_t kSlotStep = C::kSlotBytes >> 4;
-        unsigned clean_ph = 0, p_ph0 = 0, p_ph1 = 0, open0 = 0, open1 = 0;  // open: the stream's O has been written
-        int slot = 0;
+        unsigned clean_ph = 0, p_ph = 0, open = 0;  // p_ph, open: a bit per stream; open: its O has been written
+        int slot = 0, k = 0, v = 0;
         unsigned phase = 0;
         bool ok = warp_wait(smem_u32(&bar_q), 0, &gave_up);
         // K and V tiles are taken in ring order: waits for the next one, returns its slot
@@ -679,99 +708,70 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++slot == C::kSlots) slot = 0, phase ^= 1u;
           return r;
         };
-        // S of stream s from the K tile in slot k; `last`: nothing else reads that tile
-        const auto scores = [&](int s, uint32_t q, int k, bool last) {
-          fence_after();
-          if (elect()) {
-            const uint32_t a = dq + q, b = dk + k * kSlotStep;
-#pragma unroll
-            for (int i = 0; i < C::kHalves * 4; ++i)
-              mma_ss(s * 128, a + (i / 4) * 1024 + (i % 4) * 2, b + (i / 4) * 1024 + (i % 4) * 2, id_s, i > 0);
-            mma_commit(smem_u32(&bar_s[s]));
-            if (last) mma_commit(smem_u32(&bar_empty[k]));
-          }
-          __syncwarp();
-        };
-        // O of stream s from its P and the V tile in slot v, 64 keys and then the other 64, whose weights may still
-        // be on their way; `end`: the stream's last
-        const auto values = [&](int s, int v, unsigned &open, unsigned &ph, bool last, bool end) {
-          fence_after();
-          const uint32_t b = dv + v * kSlotStep;
-          if (elect()) {
-            mma_ts(256 + s * 128, s * 128, b, id_o, open);
-#pragma unroll
-            for (int i = 1; i < kTile / 32; ++i) mma_ts(256 + s * 128, s * 128 + i * 8, b + i * 128, id_o, 1);
-          }
-          __syncwarp();
-          open = 1;
-          if (!warp_wait(smem_u32(&bar_p[s][1]), ph, &gave_up)) return false;
-          ph ^= 1u;
-          fence_after();
-          if (elect()) {
-#pragma unroll
-            for (int i = kTile / 32; i < kTile / 16; ++i)
-              mma_ts(256 + s * 128, s * 128 + i * 8, b + i * 128, id_o, 1);
-            if (last) mma_commit(smem_u32(&bar_empty[v]));
-            if (end) mma_commit(smem_u32(&bar_o[s]));
-          }
-          __syncwarp();
-          return true;
-        };
-        // V tile j has landed; warps 10-11 look it over (while the softmax runs) where some row does not see all of it
-        const auto wait_v = [&](int j, int &v) {
-          if (!next(v)) return false;
-          if (j >= n_full && elect()) mbar_arrive(smem_u32(&bar_dirty));
-          __syncwarp();
-          return true;
-        };
-        const auto wait_clean = [&](int j) {
-          if (j < n_full) return true;
-          const bool r = warp_wait(smem_u32(&bar_clean), clean_ph, &gave_up);
-          clean_ph ^= 1u;
-          return r;
-        };
-        const auto wait_p = [&](int s, unsigned ph) { return warp_wait(smem_u32(&bar_p[s][0]), ph, &gave_up); };
-        int k = 0, v = 0;
-        if (ok && pairs) {
-          constexpr uint32_t kSecond = kSlotStep;  // the second Q tile
-          ok = next(k);
-          if (ok) {
-            if (n_0 > 0) scores(0, 0, k, false);
-            scores(1, kSecond, k, true);
-          }
-          for (int j = 0; ok && j < n_k; ++j) {
-            if (!(ok = wait_v(j, v))) break;
-            const bool more = j + 1 < n_k;
-            if (j < n_0 && !(ok = wait_p(0, p_ph0))) break;
-            if (!(ok = wait_clean(j))) break;
-            if (j < n_0 && !(ok = values(0, v, open0, p_ph0, false, j + 1 == n_0))) break;
-            if (more) {
-              if (!(ok = next(k))) break;
-              if (j + 1 < n_0) scores(0, 0, k, false);
+        // Step u: the product with V of key tile j, then the scores of that stream's next tile. A pair's streams
+        // share key tile j = u div 2; solo, tile j = u belongs to stream j mod 2. The first two steps only make scores.
+        const int total = pairs ? 2 * n_k : n_k;
+#pragma unroll 1
+        for (int u = -2; ok && u < total; ++u) {
+          const int s = u & 1, j = pairs ? u >> 1 : u, js = pairs ? j + 1 : j + 2;
+          const int mine = pairs && s == 0 ? n_0 : n_k;  // this stream's tiles lie before this one
+          const bool takes = !pairs || s == 0, leaves = !pairs || s == 1;
+          const uint32_t ts = s * 128, to = 256 + s * 128;
+          if (j >= 0) {
+            if (takes) {
+              if (!(ok = next(v))) break;
+              // warps 10-11 look V over (while the softmax runs) where some row does not see all of it
+              if (j >= n_full && elect()) mbar_arrive(smem_u32(&bar_dirty));
+              __syncwarp();
             }
-            if (!(ok = wait_p(1, p_ph1)) || !(ok = values(1, v, open1, p_ph1, true, !more))) break;
-            if (more) scores(1, kSecond, k, true);
-          }
-        } else if (ok) {
-          // solo: key tile j belongs to stream j mod 2
-          const auto step = [&](int j, int s, unsigned &ph, unsigned &open) {
-            if (j + 1 < n_k) {
-              if (!next(k)) return false;
-              scores(s ^ 1, 0, k, true);
+            if (j < mine && !(ok = warp_wait(smem_u32(&bar_p[s][0]), p_ph >> s & 1u, &gave_up))) break;
+            if (takes && j >= n_full) {
+              if (!(ok = warp_wait(smem_u32(&bar_clean), clean_ph, &gave_up))) break;
+              clean_ph ^= 1u;
             }
-            if (!wait_v(j, v) || !wait_p(s, ph) || !wait_clean(j)) return false;
-            return values(s, v, open, ph, true, j + 2 >= n_k);
-          };
-          ok = next(k);
-          if (ok) scores(0, 0, k, true);
-          for (int j = 0; ok && j < n_k; j += 2) {
-            ok = step(j, 0, p_ph0, open0);
-            if (ok && j + 1 < n_k) ok = step(j + 1, 1, p_ph1, open1);
+            if (j < mine) {
+              // 64 keys, and then the other 64, whose weights may still be on their way
+              fence_after();
+              const uint32_t b = dv + v * kSlotStep;
+              if (elect()) {
+                mma_ts(to, ts, b, id_o, open >> s & 1u);
+#pragma unroll
+                for (int i = 1; i < kTile / 32; ++i) mma_ts(to, ts + i * 8, b + i * 128, id_o, 1);
+              }
+              __syncwarp();
+              open |= 1u << s;
+              if (!(ok = warp_wait(smem_u32(&bar_p[s][1]), p_ph >> s & 1u, &gave_up))) break;
+              p_ph ^= 1u << s;
+              fence_after();
+              if (elect()) {
+#pragma unroll
+                for (int i = kTile / 32; i < kTile / 16; ++i) mma_ts(to, ts + i * 8, b + i * 128, id_o, 1);
+                if (leaves) mma_commit(smem_u32(&bar_empty[v]));
+                if (js >= mine) mma_commit(smem_u32(&bar_o[s]));
+              }
+              __syncwarp();
+            }
+          }
+          if (js < n_k) {
+            if (takes && !(ok = next(k))) break;
+            if (js < mine) {
+              fence_after();
+              if (elect()) {
+                const uint32_t a = dq + (pairs ? s * kSlotStep : 0), b = dk + k * kSlotStep;
+#pragma unroll
+                for (int i = 0; i < C::kHalves * 4; ++i)
+                  mma_ss(ts, a + (i / 4) * 1024 + (i % 4) * 2, b + (i / 4) * 1024 + (i % 4) * 2, id_s, i > 0);
+                mma_commit(smem_u32(&bar_s[s]));
+                if (leaves) mma_commit(smem_u32(&bar_empty[k]));
+              }
+              __syncwarp();
+            }
           }
         }
         // nothing of this CTA is in flight in the tensor core when it ends
         if (elect()) mma_commit(smem_u32(&bar_drain));
         __syncwarp();
+#pragma unroll 1
         for (unsigned i = 0; i < kWaitLimit; ++i) {
           if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar_drain), 0))) break;
           __nanosleep(32);
@@ -912,78 +912,81 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (first < first_masked) first += (first_masked - first + step - 1) / step * step;
       add_not_finite<HDP>(p, w.s, t0, kvh, tok, tok0, tok1, w.ta + first, w.ta + (pair ? mine : nk), step, to);
     }
-    float *joined = reinterpret_cast<float *>(raw + (ring - smem_u32(raw)));  // [HDP][128], over the ring
-
-    if (!pair) {
-      // solo: stream 1's maximum, sum and O go through shared memory; both streams' matrix work is done first
+    // Solo: the two streams' sums over the same rows are joined through shared memory (over the ring, whose last tile
+    // both have waited for): each stream hands over the half of its columns that the other one finishes.
+    constexpr int kHalf = HDP / 2;
+    float *joined = reinterpret_cast<float *>(raw + (ring - smem_u32(raw)));  // [HDP][128]
+    float *join = joined + HDP * kTile;  // maximum and sum of each stream's rows
+    const bool second = !pair && nk > 1;
+    float a0 = 1.f, a1 = 0.f;
+    if (second) {
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (s == 1) {
-        join[0][row] = m;
-        join[1][row] = l;
-        if (active && ok && mine > 0)
+      join[2 * s * kTile + row] = m;
+      join[(2 * s + 1) * kTile + row] = l;
+      if (active && ok) {
 #pragma unroll 1
-          for (int c = 0; c < HDP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(to + 32 * c, o);
-            tmem_wait_ld();
+        for (int c = 0; c < kHalf; c += 16) {
+          const int col = (1 - s) * kHalf + c;
+          uint32_t o[16];
+          tmem_ld16(to + col, o);
+          tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) joined[(32 * c + i) * kTile + row] = __uint_as_float(o[i]);
-          }
+          for (int i = 0; i < 16; ++i) joined[(col + i) * kTile + row] = __uint_as_float(o[i]);
+        }
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
+      const float m1 = join[(2 - 2 * s) * kTile + row], mm = fmaxf(m, m1);
+      const float ref = mm == -INFINITY ? 0.f : mm;
+      a0 = ex2(m - ref);
+      a1 = ex2(m1 - ref);
+      l = l * a0 + join[(3 - 2 * s) * kTile + row] * a1;
+      m = mm;
     }
-    if ((pair || s == 0) && active && ok) {
-      float a0 = 1.f, a1 = 0.f;
-      const bool second = !pair && nk > 1;
-      if (second) {
-        const float m1 = join[0][row], mm = fmaxf(m, m1);
-        const float ref = mm == -INFINITY ? 0.f : mm;
-        a0 = ex2(m - ref);
-        a1 = ex2(m1 - ref);
-        l = l * a0 + join[1][row] * a1;
-        m = mm;
-      }
+    if ((pair || s == 0 || second) && active && ok) {
       const bool valid = row < rows;
       const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-      const int64_t unit = (static_cast<int64_t>(rest) * p.d.nkv + kvh) * p.tpi + tile;
+      a0 *= inv;
+      a1 *= inv;
+      const int64_t unit = ((static_cast<int64_t>(item) * p.splits + split) * p.d.nkv + kvh) * p.tpi + tile;
       float *part = p.workspace + unit * (kTile * (HDP + 2));
       const int64_t token = w.s.q0 + t0 + tok;
       uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
                       static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
+      const int c_end = second ? (s + 1) * kHalf : HDP;
 #pragma unroll 1
-      for (int c = 0; c < HDP / 32; ++c) {
-        float o[32];
+      for (int c = second ? s * kHalf : 0; c < c_end; c += 16) {
+        float o[16];
         if (mine > 0) {
-          tmem_ld32(to + 32 * c, reinterpret_cast<uint32_t *>(o));
+          tmem_ld16(to + c, reinterpret_cast<uint32_t *>(o));
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          for (int i = 0; i < 16; ++i) o[i] = 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (second) o[i] = o[i] * a0 + joined[(32 * c + i) * kTile + row] * a1;
-          o[i] *= inv;
+        for (int i = 0; i < 16; ++i) {
+          o[i] *= a0;
+          if (second) o[i] += joined[(c + i) * kTile + row] * a1;
         }
         if (!valid) continue;
         if (p.splits > 1) {
           if (mine == 0) continue;  // the sum of zero written below says that there is nothing
 #pragma unroll
-          for (int i = 0; i < 32; ++i) part[(32 * c + i) * kTile + row] = o[i];
+          for (int i = 0; i < 16; ++i) part[(c + i) * kTile + row] = o[i];
         } else if (p.vec_out) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (32 * c + i < p.d.hd)
-              *reinterpret_cast<uint4 *>(out + 32 * c + i) =
+          for (int i = 0; i < 16; i += 8)
+            if (c + i < p.d.hd)
+              *reinterpret_cast<uint4 *>(out + c + i) =
                   make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]),
                              pack_bf16(o[i + 6], o[i + 7]));
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i < p.d.hd) out[32 * c + i] = f2b(o[i]);
+          for (int i = 0; i < 16; ++i)
+            if (c + i < p.d.hd) out[c + i] = f2b(o[i]);
         }
       }
-      if (p.splits > 1 && valid) {
+      if (p.splits > 1 && valid && (pair || s == 0)) {
         part[HDP * kTile + row] = m;
         part[(HDP + 1) * kTile + row] = l;
       }
@@ -999,21 +1002,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the shares of the key axis: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
-// A block takes 32 rows of one tile: the weights of all shares first, then a
-// warp for 8 columns, a lane for a row.
-constexpr int kMaxSplits = 64;
+// A block takes 32 rows and 32 columns of one tile: the weights of all shares
+// first, then a warp for 8 columns, a lane for a row, the loads of 8 shares at
+// once (one after the other they are all this kernel waits for).
+constexpr int kMaxSplits = 64, kJoinThreads = 128, kJoinBatch = 8;
 
 template <int HDP>
-__global__ void __launch_bounds__(HDP * 4) attn_join_kernel(const __grid_constant__ TcParams p) {
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ TcParams p) {
   __shared__ float weight[kMaxSplits][32], sums[kMaxSplits][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int u = blockIdx.x;
-  const int quarter = u % 4;
-  u /= 4;
-  const int tile = u % p.tpi;
-  u /= p.tpi;
-  const int kvh = u % p.d.nkv;
-  const int item = u / p.d.nkv;
+  const int item = blockIdx.x, kvh = blockIdx.y, quarter = blockIdx.z & 3, tile = blockIdx.z / 4 % p.tpi;
+  const int c0 = (blockIdx.z / 4 / p.tpi) * 32 + warp * 8;
   const Item w = make_item(p, item, 0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!w.live) return;
@@ -1023,26 +1022,38 @@ __global__ void __launch_bounds__(HDP * 4) attn_join_kernel(const __grid_constan
   const bool valid = row < rows;
   const int64_t share = static_cast<int64_t>(p.d.nkv) * p.tpi * (kTile * (HDP + 2));
   const float *part = p.workspace + (static_cast<int64_t>(item) * p.splits * p.d.nkv * p.tpi + kvh * p.tpi + tile) *
-                                          (kTile * (HDP + 2));
+                                        (kTile * (HDP + 2));
   // shares that the item's key tiles do not reach are not read; every other CTA wrote its rows in full
-  for (int sp = warp; sp < w.shares; sp += HDP / 8) {
+#pragma unroll 1
+  for (int sp = warp; sp < w.shares; sp += kJoinThreads / 32) {
     weight[sp][lane] = valid ? part[sp * share + HDP * kTile + row] : -INFINITY;
     sums[sp][lane] = valid ? part[sp * share + (HDP + 1) * kTile + row] : 0.f;
   }
   __syncthreads();
-  const int c0 = warp * 8;
   if (!valid || c0 >= p.d.hd) return;
   float m = -INFINITY;
+#pragma unroll 4
   for (int sp = 0; sp < w.shares; ++sp) m = fmaxf(m, weight[sp][lane]);
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[8] = {};
   const float *q = part + c0 * kTile + row;
-#pragma unroll 4
-  for (int sp = 0; sp < w.shares; ++sp) {
-    const float a = ex2(weight[sp][lane] - ref);
-    l += a * sums[sp][lane];
+#pragma unroll 1
+  for (int s0 = 0; s0 < w.shares; s0 += kJoinBatch) {
+    float x[kJoinBatch][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] += a * q[sp * share + i * kTile];
+    for (int b = 0; b < kJoinBatch; ++b) {
+      const float *r = q + min(s0 + b, w.shares - 1) * share;  // behind the last share: again the last, not added
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[b][i] = __ldcg(r + i * kTile);
+    }
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b) {
+      if (s0 + b >= w.shares) break;
+      const float a = ex2(weight[s0 + b][lane] - ref);
+      l += a * sums[s0 + b][lane];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] += a * x[b][i];
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -1123,7 +1134,7 @@ static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 // the rest.
 static bool tensor_cores(const aib_attn_desc &d, bool tree) {
   const int64_t b = tree ? d.batch : 1, kb = tree || d.len_k ? d.batch : 1;
-  return d.hd % 8 == 0 && d.hd <= 128 && d.nh / d.nkv <= kTile && d.scale > 0.f && d.key_rows > 0 && aligned16(d.q) &&
+  return d.hd % 8 == 0 && d.hd <= 128 && d.nh / d.nkv <= kTile && d.nkv <= 65535 && d.scale > 0.f && d.key_rows > 0 && aligned16(d.q) &&
          aligned16(d.k) && aligned16(d.v) && tma_stride(d.tokens, d.q_token_stride) &&
          tma_stride(d.nh, d.q_head_stride) && tma_stride(b, d.q_batch_stride) &&
          tma_stride(d.key_rows, d.k_token_stride) && tma_stride(d.nkv, d.k_head_stride) &&
@@ -1206,16 +1217,16 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
               d.out_batch_stride % 8 == 0;
   p.workspace = workspace;
   p.status = status;
-  const int64_t grid = pl.items * pl.splits * d.nkv;
-  attn_tc_kernel<HDP><<<static_cast<unsigned>(grid), kThreads, Cfg<HDP>::kSmem, st>>>(mq, mk, mv, p);
+  const dim3 grid(static_cast<unsigned>(pl.items * d.nkv), static_cast<unsigned>(pl.splits));
+  attn_tc_kernel<HDP><<<grid, kThreads, Cfg<HDP>::kSmem, st>>>(mq, mk, mv, p);
   if ((e = cudaGetLastError()) == cudaSuccess && pl.splits > 1) {
     // started while the last shares still run (it waits for them before it reads)
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(pl.items * d.nkv * pl.tpi * 4));
-    cfg.blockDim = dim3(HDP * 4);
+    cfg.gridDim = dim3(static_cast<unsigned>(pl.items), static_cast<unsigned>(d.nkv), 4 * pl.tpi * (HDP / 32));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
