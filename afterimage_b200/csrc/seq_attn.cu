@@ -215,6 +215,7 @@ struct Cfg {
 struct TcParams {
   aib_attn_desc d;
   int group, tt;       // heads per kv head, tokens per tile
+  int group_rcp;       // r / group is r * group_rcp >> 16 for r < 128
   int tpi;             // tiles an item may hold: 2 or 1
   int splits;          // shares of the key axis
   int items;           // upper bound of the items
@@ -236,18 +237,11 @@ struct Item {
   bool live;
 };
 
-// Items of sequence i (`unit` tokens each).
+// Items of sequence i.
 __device__ __forceinline__ int items_of(const TcParams &p, int i) {
   const int unit = p.tt * p.tpi;
   const int q0 = cut(p.d.cu_q[i], 0, p.d.tokens);
   return (cut(p.d.cu_q[i + 1], q0, p.d.tokens) - q0 + unit - 1) / unit;
-}
-// F(l) of find_item. Collective over the warp.
-__device__ __forceinline__ int items_at_or_above(const TcParams &p, int l) {
-  int f = 0;
-#pragma unroll 1
-  for (int i = threadIdx.x & 31; i < static_cast<int>(p.d.batch); i += 32) f += max(0, items_of(p, i) - l);
-  return __reduce_add_sync(0xffffffffu, f);
 }
 
 // Item number -> sequence and first tile. Prompts: items are numbered from
@@ -258,18 +252,32 @@ __device__ __forceinline__ int items_at_or_above(const TcParams &p, int l) {
 // Collective over the warp.
 __device__ __forceinline__ bool find_among_prompts(const TcParams &p, int item, int &b, int &level) {
   const int lane = threadIdx.x & 31, batch = static_cast<int>(p.d.batch);
-  if (items_at_or_above(p, 0) <= item) return false;
-  int lo = 0, hi = static_cast<int>(p.d.tokens);  // F(lo) > item >= F(hi)
+  const int first = lane < batch ? items_of(p, lane) : 0;  // up to 32 sequences need no second read
+  int lo = 0, hi = __reduce_max_sync(0xffffffffu, first);
+  int all = __reduce_add_sync(0xffffffffu, first);
+#pragma unroll 1
+  for (int i = lane + 32; i - lane < batch; i += 32) {
+    const int n = i < batch ? items_of(p, i) : 0;
+    hi = max(hi, __reduce_max_sync(0xffffffffu, n));
+    all += __reduce_add_sync(0xffffffffu, n);
+  }
+  if (all <= item) return false;
+  int above = 0;  // F(hi); F(lo) > item >= F(hi)
 #pragma unroll 1
   while (hi - lo > 1) {
-    const int mid = lo + (hi - lo) / 2;
-    if (items_at_or_above(p, mid) > item) lo = mid; else hi = mid;
+    const int mid = (lo + hi) >> 1;
+    int f = max(0, first - mid);
+#pragma unroll 1
+    for (int i = lane + 32; i < batch; i += 32) f += max(0, items_of(p, i) - mid);
+    f = __reduce_add_sync(0xffffffffu, f);
+    if (f > item) lo = mid; else hi = mid, above = f;
   }
-  int rank = item - items_at_or_above(p, lo + 1);  // among the sequences that reach this level
+  int rank = item - above;  // among the sequences that reach level lo (hi = lo + 1)
   level = lo;
 #pragma unroll 1
   for (int i0 = 0; i0 < batch; i0 += 32) {
-    unsigned has = __ballot_sync(0xffffffffu, i0 + lane < batch && items_of(p, i0 + lane) > lo);
+    const int n = i0 == 0 ? first : (i0 + lane < batch ? items_of(p, i0 + lane) : 0);
+    unsigned has = __ballot_sync(0xffffffffu, n > lo);
     if (rank < __popc(has)) {
 #pragma unroll 1
       for (; rank > 0; --rank) has &= has - 1;
@@ -497,6 +505,16 @@ __device__ __forceinline__ float max_nan3(float a, float b, float c) {
 
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&x)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 x) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+
 // bits of the seen keys among the four 32-key words of key tile t, for this
 // thread's row (token tok of the tile; first token of the tile is ti within
 // the sequence). Collective over the warp for trees.
@@ -711,22 +729,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Step u: the product with V of key tile j, then the scores of that stream's next tile. A pair's streams
         // share key tile j = u div 2; solo, tile j = u belongs to stream j mod 2. The first two steps only make scores.
         const int total = pairs ? 2 * n_k : n_k;
-#pragma unroll 1
-        for (int u = -2; ok && u < total; ++u) {
-          const int s = u & 1, j = pairs ? u >> 1 : u, js = pairs ? j + 1 : j + 2;
+        // (two steps to an iteration: the streams' addresses are constants then)
+        const auto step = [&](const int u, const int s) {
+          const int j = pairs ? u >> 1 : u, js = pairs ? j + 1 : j + 2;
           const int mine = pairs && s == 0 ? n_0 : n_k;  // this stream's tiles lie before this one
           const bool takes = !pairs || s == 0, leaves = !pairs || s == 1;
           const uint32_t ts = s * 128, to = 256 + s * 128;
           if (j >= 0) {
             if (takes) {
-              if (!(ok = next(v))) break;
+              if (!next(v)) return false;
               // warps 10-11 look V over (while the softmax runs) where some row does not see all of it
               if (j >= n_full && elect()) mbar_arrive(smem_u32(&bar_dirty));
               __syncwarp();
             }
-            if (j < mine && !(ok = warp_wait(smem_u32(&bar_p[s][0]), p_ph >> s & 1u, &gave_up))) break;
+            if (j < mine && !warp_wait(smem_u32(&bar_p[s][0]), p_ph >> s & 1u, &gave_up)) return false;
             if (takes && j >= n_full) {
-              if (!(ok = warp_wait(smem_u32(&bar_clean), clean_ph, &gave_up))) break;
+              if (!warp_wait(smem_u32(&bar_clean), clean_ph, &gave_up)) return false;
               clean_ph ^= 1u;
             }
             if (j < mine) {
@@ -740,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               __syncwarp();
               open |= 1u << s;
-              if (!(ok = warp_wait(smem_u32(&bar_p[s][1]), p_ph >> s & 1u, &gave_up))) break;
+              if (!warp_wait(smem_u32(&bar_p[s][1]), p_ph >> s & 1u, &gave_up)) return false;
               p_ph ^= 1u << s;
               fence_after();
               if (elect()) {
@@ -753,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (js < n_k) {
-            if (takes && !(ok = next(k))) break;
+            if (takes && !next(k)) return false;
             if (js < mine) {
               fence_after();
               if (elect()) {
@@ -767,6 +785,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
             }
           }
+          return true;
+        };
+#pragma unroll 1
+        for (int u = -2; ok && u < total; u += 2) {
+          ok = step(u, 0);
+          if (ok && u + 1 < total) ok = step(u + 1, 1);
         }
         // nothing of this CTA is in flight in the tensor core when it ends
         if (elect()) mma_commit(smem_u32(&bar_drain));
@@ -785,23 +809,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!warp_wait(smem_u32(&bar_dirty), (j - first_masked) & 1u, &gave_up)) break;
         const uint32_t base = ring + (pos_v(j) % C::kSlots) * C::kSlotBytes;
         const int rows_seen = seen_end - (w.ta + j) * kTile;
+        // a value times zero is zero unless it is not finite: one multiply-add for two values finds whether any is
+        const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+        __nv_bfloat162 any = zero;
 #pragma unroll 4
         for (int e = self; e < C::kSlotBytes / 16; e += 64) {
           uint32_t x[4];
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                       : "r"(base + e * 16)
-                       : "memory");
-          bool found = false;
+          lds128(base + e * 16, x);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (not_finite_bf16(x[i])) x[i] &= 0xffff0000u, found = true;
-            if (not_finite_bf16(x[i] >> 16)) x[i] &= 0x0000ffffu, found = true;
-          }
-          if (found) {
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + e * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
-                         "r"(x[3])
-                         : "memory");
+          for (int i = 0; i < 4; ++i) any = __hfma2(*reinterpret_cast<__nv_bfloat162 *>(&x[i]), zero, any);
+        }
+        if (__hisnan(any.x) || __hisnan(any.y)) {
+#pragma unroll 1
+          for (int e = self; e < C::kSlotBytes / 16; e += 64) {
+            uint32_t x[4];
+            lds128(base + e * 16, x);
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (not_finite_bf16(x[i])) x[i] &= 0xffff0000u, found = true;
+              if (not_finite_bf16(x[i] >> 16)) x[i] &= 0x0000ffffu, found = true;
+            }
+            if (!found) continue;
+            sts128(base + e * 16, make_uint4(x[0], x[1], x[2], x[3]));
             if ((e % 1024) / 8 < rows_seen) bad_seen = 1;
           }
         }
@@ -820,8 +850,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wrow = (warp & 3) * 32, row = wrow + lane;
     const int rows = cnt * p.group;
     const bool active = wrow < rows;  // a warp without rows only keeps the barriers going
-    const int tok = min(row / p.group, cnt - 1);
-    const int tok0 = wrow / p.group, tok1 = min((wrow + 31) / p.group, cnt - 1);
+    const int tok = min((row * p.group_rcp) >> 16, cnt - 1);
+    const int tok0 = (wrow * p.group_rcp) >> 16, tok1 = min(((wrow + 31) * p.group_rcp) >> 16, cnt - 1);
     const uint32_t lanes = static_cast<uint32_t>(wrow) << 16;
     const uint32_t ts = s * 128 + lanes, to = 256 + s * 128 + lanes;
     const float sl = p.scale_log2;
@@ -949,9 +979,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       a1 *= inv;
       const int64_t unit = ((static_cast<int64_t>(item) * p.splits + split) * p.d.nkv + kvh) * p.tpi + tile;
       float *part = p.workspace + unit * (kTile * (HDP + 2));
-      const int64_t token = w.s.q0 + t0 + tok;
-      uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride + token * p.d.out_token_stride +
-                      static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
+      uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride +
+                      static_cast<int64_t>(w.s.q0 + t0) * p.d.out_token_stride +
+                      static_cast<int64_t>(kvh * p.group) * p.d.out_head_stride;  // the tile's first row
+      const uint32_t stage = smem_q + s * C::kSlotBytes + wrow * (2 * HDP);  // 32 rows of HDP values
       const int c_end = second ? (s + 1) * kHalf : HDP;
 #pragma unroll 1
       for (int c = second ? s * kHalf : 0; c < c_end; c += 16) {
@@ -968,22 +999,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           o[i] *= a0;
           if (second) o[i] += joined[(c + i) * kTile + row] * a1;
         }
-        if (!valid) continue;
         if (p.splits > 1) {
-          if (mine == 0) continue;  // the sum of zero written below says that there is nothing
+          if (mine == 0 || !valid) continue;  // (the sum of zero written below says that there is nothing)
 #pragma unroll
           for (int i = 0; i < 16; ++i) part[(c + i) * kTile + row] = o[i];
-        } else if (p.vec_out) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 8)
-            if (c + i < p.d.hd)
-              *reinterpret_cast<uint4 *>(out + c + i) =
-                  make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]),
-                             pack_bf16(o[i + 6], o[i + 7]));
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < p.d.hd) out[c + i] = f2b(o[i]);
+          for (int i = 0; i < 16; i += 8)
+            sts128(stage + lane * (2 * HDP) + ((((c + i) / 8) ^ (lane & 7)) * 16),
+                   make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]),
+                              pack_bf16(o[i + 6], o[i + 7])));
+        }
+      }
+      if (p.splits == 1) {
+        // a thread holds a row: written as they are, every store of a warp would touch 32 lines. Through the warp's
+        // part of the Q tile (nothing reads it any more) a row's 16-byte pieces go out together.
+        __syncwarp();
+        const int per = second ? kHalf / 8 : HDP / 8;  // pieces of a row; a power of two
+        const int first = second ? s * per : 0;
+#pragma unroll 4
+        for (int e = lane; e < 32 * per; e += 32) {
+          const int r = e / per, q = first + e % per;
+          if (wrow + r >= rows || q * 8 >= p.d.hd) continue;
+          const int to_tok = ((wrow + r) * p.group_rcp) >> 16;
+          uint16_t *to_row = out + to_tok * p.d.out_token_stride +
+                             static_cast<int64_t>(wrow + r - to_tok * p.group) * p.d.out_head_stride + q * 8;
+          uint32_t x[4];
+          lds128(stage + r * (2 * HDP) + ((q ^ (r & 7)) * 16), x);
+          if (p.vec_out) {
+            *reinterpret_cast<uint4 *>(to_row) = make_uint4(x[0], x[1], x[2], x[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to_row[i] = static_cast<uint16_t>(x[i / 2] >> (16 * (i & 1)));
+          }
         }
       }
       if (p.splits > 1 && valid && (pair || s == 0)) {
@@ -1208,6 +1256,7 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   TcParams p;
   p.d = d;
   p.group = pl.group;
+  p.group_rcp = (65536 + pl.group - 1) / pl.group;
   p.tt = pl.tt;
   p.tpi = pl.tpi;
   p.splits = pl.splits;
