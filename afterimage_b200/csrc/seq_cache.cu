@@ -51,8 +51,101 @@ __device__ __forceinline__ int64_t find_sequence(const int64_t *cu, int64_t batc
   return lo;
 }
 
-// One block per token: its angles once, then a warp per head. Row values in
-// fp32 (norm, rotation), one rounding at the write.
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  return static_cast<uint32_t>(f2b(hi)) << 16 | f2b(lo);
+}
+__device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+
+// Head sizes 16 LPR (64, 128, 256) with everything on 16-byte boundaries. One
+// block per token; LPR lanes to a head, a lane with eight values of the first
+// half and their eight partners of the second, so that the rotation stays in
+// the lane and the norm takes log2(LPR) shuffles. Bound by memory: the rows
+// are asked for before the block looks up its sequence and makes its angles
+// (a chain of loads of its own), two rows to a thread at once. 8192 tokens of
+// 48 heads of 128 (201 MB): MEASURED_LARGE; 26 tokens: MEASURED_SMALL.
+template <int LPR>
+__global__ void __launch_bounds__(256) rope_cache_vec_kernel(const RopeParams p) {
+  constexpr int kHalf = 8 * LPR, kHd = 16 * LPR, kRows = 256 / LPR, kAtOnce = 2;
+  __shared__ __align__(16) float cs[kHalf], sn[kHalf];
+  const int64_t n = blockIdx.x;
+  const int l = threadIdx.x % LPR, r = threadIdx.x / LPR;
+  const int heads = p.nh + 2 * p.nkv;
+  const uint16_t *x = p.qkv + n * p.qkv_stride + 8 * l;
+  uint4 lo[kAtOnce], hi[kAtOnce];
+  const auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int h = h0 + i * kRows + r;
+      if (h < heads) {
+        lo[i] = *reinterpret_cast<const uint4 *>(x + static_cast<int64_t>(h) * kHd);
+        hi[i] = *reinterpret_cast<const uint4 *>(x + static_cast<int64_t>(h) * kHd + kHalf);
+      }
+    }
+  };
+  load(0);
+  const float f = threadIdx.x < kHalf ? p.inv_freq[threadIdx.x] : 0.f;
+  const int64_t depth = p.depth ? p.depth[n] : 0;
+  const int64_t b = find_sequence(p.cu, p.batch, n);
+  if (b < 0) return;  // uniform over the block
+  const int64_t first = p.start[b], at = n - p.cu[b];
+  const int64_t slot = first + at, place = first + (p.depth ? depth : at);
+  const bool in_cache = slot >= 0 && slot < p.max_len;
+  if (threadIdx.x < kHalf) turn(place, f, cs[threadIdx.x], sn[threadIdx.x]);
+  __syncthreads();
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = cs[8 * l + i], s[i] = sn[8 * l + i];
+  for (int h0 = 0; h0 < heads; h0 += kAtOnce * kRows) {
+    if (h0) load(h0);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int h = h0 + i * kRows + r;
+      const bool is_q = h < p.nh, is_k = !is_q && h < p.nh + p.nkv;
+      float u[8], v[8];
+      unpack(lo[i], u);
+      unpack(hi[i], v);
+      if (p.qn) {  // every lane of a warp takes part in the sums
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss += u[k] * u[k] + v[k] * v[k];
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float norm = rsqrtf(ss / static_cast<float>(kHd) + p.eps);
+        if (is_q || is_k) {
+          const uint16_t *w = (is_q ? p.qn : p.kn) + 8 * l;
+          float wu[8], wv[8];
+          unpack(*reinterpret_cast<const uint4 *>(w), wu);
+          unpack(*reinterpret_cast<const uint4 *>(w + kHalf), wv);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) u[k] *= norm * wu[k], v[k] *= norm * wv[k];
+        }
+      }
+      if (h >= heads || (!is_q && !in_cache)) continue;
+      uint16_t *o = is_q   ? p.q_out + (n * p.nh + h) * kHd
+                    : is_k ? p.k + b * p.k_bs + (h - p.nh) * p.k_hs + slot * p.k_ts
+                           : p.v + b * p.v_bs + (h - p.nh - p.nkv) * p.v_hs + slot * p.v_ts;
+      uint4 a = lo[i], z = hi[i];
+      if (is_q || is_k) {
+        uint32_t *aw = reinterpret_cast<uint32_t *>(&a), *zw = reinterpret_cast<uint32_t *>(&z);
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          aw[k / 2] = pack(u[k] * c[k] - v[k] * s[k], u[k + 1] * c[k + 1] - v[k + 1] * s[k + 1]);
+          zw[k / 2] = pack(v[k] * c[k] + u[k] * s[k], v[k + 1] * c[k + 1] + u[k + 1] * s[k + 1]);
+        }
+      }
+      *reinterpret_cast<uint4 *>(o + 8 * l) = a;
+      *reinterpret_cast<uint4 *>(o + 8 * l + kHalf) = z;
+    }
+  }
+}
+
+// Every other head size and alignment. One block per token: its angles once,
+// then a warp per head. Row values in fp32 (norm, rotation), one rounding at
+// the write.
 __global__ void rope_cache_kernel(const RopeParams p) {
   extern __shared__ float cs[];  // cos[half], sin[half]
   const int64_t n = blockIdx.x;
@@ -138,6 +231,39 @@ __global__ void keep_rows_kernel(const __grid_constant__ KeepParams p) {
   }
 }
 
+// The common case, an accepted path of a few rows: a warp takes one head's
+// rows of one tensor and holds them all in registers between its reads and
+// its writes (no other warp touches them), so nothing but the chain position
+// -> row -> write is waited for.
+constexpr int kKeepHeld = 8;  // units of a row that a lane holds
+
+template <typename T>
+__global__ void __launch_bounds__(256) keep_few_rows_kernel(const __grid_constant__ KeepParams p, int nkv) {
+  const int head = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (head >= nkv) return;
+  const int64_t b = blockIdx.z;
+  T *base = static_cast<T *>(p.t[blockIdx.y]) + b * p.bs + head * p.hs;
+  const int64_t pos = p.pos[b];
+  const int64_t *keep = p.keep + b * p.n;
+  T held[kKeepHeld];
+  T *to[kKeepHeld];
+#pragma unroll
+  for (int k = 0; k < kKeepHeld; ++k) {
+    const int e = lane + 32 * k, i = e / p.cols, c = e - i * p.cols;
+    to[k] = nullptr;
+    if (i >= p.n) continue;
+    const int64_t s = keep[i], src = pos + s, dst = pos + i;
+    if (s >= 0 && s != i && src >= 0 && src < p.max_len && dst >= 0 && dst < p.max_len) {
+      held[k] = base[src * p.ts + c];
+      to[k] = base + dst * p.ts + c;
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < kKeepHeld; ++k)
+    if (to[k]) *to[k] = held[k];
+}
+
 template <typename T>
 static cudaError_t launch_keep(KeepParams p, int tensors, int64_t batch, int nkv, int hd, int64_t bs, int64_t hs,
                                int64_t ts, cudaStream_t st) {
@@ -147,6 +273,11 @@ static cudaError_t launch_keep(KeepParams p, int tensors, int64_t batch, int nkv
   p.hs = hs / per;
   p.ts = ts / per;
   p.slice = p.cols;
+  if (static_cast<int64_t>(p.n) * p.cols <= 32 * kKeepHeld) {
+    const dim3 few(static_cast<unsigned>((nkv + 7) / 8), static_cast<unsigned>(tensors), static_cast<unsigned>(batch));
+    keep_few_rows_kernel<T><<<few, 256, 0, st>>>(p, nkv);
+    return cudaGetLastError();
+  }
   while (static_cast<int64_t>(p.slice) * p.n * sizeof(T) > kKeepBytes) p.slice = (p.slice + 1) / 2;
   const int slices = (p.cols + p.slice - 1) / p.slice;
   const dim3 grid(static_cast<unsigned>(nkv * slices), static_cast<unsigned>(tensors), static_cast<unsigned>(batch));
@@ -192,8 +323,20 @@ AIB_API int aib_rope_cache_packed_bf16(const void *qkv, int64_t qkv_stride, int6
   p.nkv = nkv;
   p.hd = hd;
   p.eps = eps;
-  rope_cache_kernel<<<static_cast<unsigned>(n), 256, static_cast<size_t>(hd) * sizeof(float),
-                      static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(n);
+  const uintptr_t low = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) |
+                        reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+                        reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w) |
+                        static_cast<uintptr_t>(qkv_stride | p.k_bs | p.k_hs | p.k_ts | p.v_bs | p.v_hs | p.v_ts) * 2;
+  if (low % 16 == 0 && hd == 64)
+    rope_cache_vec_kernel<4><<<grid, 256, 0, st>>>(p);
+  else if (low % 16 == 0 && hd == 128)
+    rope_cache_vec_kernel<8><<<grid, 256, 0, st>>>(p);
+  else if (low % 16 == 0 && hd == 256)
+    rope_cache_vec_kernel<16><<<grid, 256, 0, st>>>(p);
+  else
+    rope_cache_kernel<<<grid, 256, static_cast<size_t>(hd) * sizeof(float), st>>>(p);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return aib_set_errorf("rope_cache_packed: %s", cudaGetErrorString(e)), AIB_ECUDA;
   return AIB_OK;
