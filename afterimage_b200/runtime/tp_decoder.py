@@ -219,13 +219,23 @@ def _rotate_half(x: torch.Tensor) -> torch.Tensor:
 
 
 class KVCache:
-    """Static per-rank cache: [layers][2] tensors of [1, kv_heads_local, max_len, head_dim]."""
+    """Static per-rank cache: [layers][2] tensors of [batch, kv_heads_local, max_len, head_dim]. `lengths` counts the
+    tokens of each sequence; `length` is the first one's (the only one's, where a forward takes a single sequence)."""
 
-    def __init__(self, n_layers, kv_heads, head_dim, max_len, device, dtype=torch.bfloat16):
-        self.k = [torch.zeros(1, kv_heads, max_len, head_dim, device=device, dtype=dtype) for _ in range(n_layers)]
-        self.v = [torch.zeros(1, kv_heads, max_len, head_dim, device=device, dtype=dtype) for _ in range(n_layers)]
+    def __init__(self, n_layers, kv_heads, head_dim, max_len, device, dtype=torch.bfloat16, batch=1):
+        shape = (batch, kv_heads, max_len, head_dim)
+        self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(n_layers)]
+        self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(n_layers)]
         self.max_len = max_len
-        self.length = 0
+        self.lengths = [0] * batch
+
+    @property
+    def length(self) -> int:
+        return self.lengths[0]
+
+    @length.setter
+    def length(self, n: int) -> None:
+        self.lengths[0] = n
 
 
 class _StepState:
@@ -504,6 +514,176 @@ class TPDecoder:
                 self.timeline.append(("compute", i, t0, _mark(torch.cuda.current_stream(self.device))))
         return tp_ops.add_rmsnorm(x, delta, self.weight("model.norm.weight"), self.eps)
 
+    def _layers_rows(self, x: torch.Tensor, cache: KVCache, cu: list, start: list, depth, attend,
+                     attend_plain) -> torch.Tensor:
+        """Every layer for packed rows x [N, H] (sequence b: rows cu[b] ..
+        cu[b + 1] - 1, written to its cache from row start[b] on), then the
+        final norm. `attend(i, q)` is the layer's attention over the caches,
+        q [N, nh, hd] -> the same; `attend_plain` the same in torch, for the
+        unfused mode. `depth`: seq_ops.rope_cache_packed's."""
+        if not self.fused:
+            return self._layers_rows_plain(x, cache, cu, start, depth, attend_plain)
+        from . import seq_ops, tp_ops
+        dev = self.device
+        d_cu = torch.tensor(cu, dtype=torch.int64, device=dev)
+        d_start = torch.tensor(start, dtype=torch.int64, device=dev)
+        n = x.shape[0]
+        x = x.contiguous()
+        delta = None
+        for i in range(self.n_layers):
+            W = self.layer_weights(i)
+            t0 = _mark(torch.cuda.current_stream(dev)) if self.timeline is not None else None
+            h = tp_ops.add_rmsnorm(x, delta, W["input_layernorm.weight"], self.eps)
+            qkv = F.linear(h, self._joined(W, *self.JOINS[0]))
+            q = seq_ops.rope_cache_packed(qkv, self.nh, self.nkv, self.hd, d_cu, d_start, self.inv_freq, cache.k[i],
+                                          cache.v[i], depth=depth,
+                                          q_norm=W.get("self_attn.q_norm.weight") if self.qk_norm else None,
+                                          k_norm=W.get("self_attn.k_norm.weight") if self.qk_norm else None,
+                                          eps=self.eps)
+            o = self._row_parallel(attend(i, q).reshape(n, -1), W["self_attn.o_proj.weight"])
+            h = tp_ops.add_rmsnorm(x, o.contiguous(), W["post_attention_layernorm.weight"], self.eps)
+            m = tp_ops.silu_mul(self._proj(h, self._joined(W, *self.JOINS[1])))
+            delta = self._row_parallel(m, W["mlp.down_proj.weight"]).contiguous()
+            if t0 is not None:
+                self.timeline.append(("compute", i, t0, _mark(torch.cuda.current_stream(dev))))
+        return tp_ops.add_rmsnorm(x, delta, self.weight("model.norm.weight"), self.eps)
+
+    def _layers_rows_plain(self, x, cache, cu, start, depth, attend):
+        n = x.shape[0]
+        seq = torch.zeros(n, dtype=torch.long, device=x.device)
+        slot = torch.zeros(n, dtype=torch.long, device=x.device)
+        for b, s in enumerate(start):
+            seq[cu[b]:cu[b + 1]] = b
+            slot[cu[b]:cu[b + 1]] = torch.arange(s, s + cu[b + 1] - cu[b], device=x.device)
+        place = slot if depth is None else torch.tensor(start, device=x.device)[seq] + depth
+        cos, sin = self._rope(place, x.dtype)
+        cos, sin = cos[:, None], sin[:, None]
+        for i in range(self.n_layers):
+            W = self.layer_weights(i)
+            h = _rms_norm(x, W["input_layernorm.weight"], self.eps)
+            q = F.linear(h, W["self_attn.q_proj.weight"]).view(n, self.nh, self.hd)
+            k = F.linear(h, W["self_attn.k_proj.weight"]).view(n, self.nkv, self.hd)
+            v = F.linear(h, W["self_attn.v_proj.weight"]).view(n, self.nkv, self.hd)
+            if self.qk_norm:
+                q = _rms_norm(q, W["self_attn.q_norm.weight"], self.eps)
+                k = _rms_norm(k, W["self_attn.k_norm.weight"], self.eps)
+            q = q * cos + _rotate_half(q) * sin
+            cache.k[i][seq, :, slot] = k * cos + _rotate_half(k) * sin
+            cache.v[i][seq, :, slot] = v
+            a = attend(i, q).reshape(n, self.nh * self.hd)
+            x = x + self._row_parallel(a, W["self_attn.o_proj.weight"])
+            h = _rms_norm(x, W["post_attention_layernorm.weight"], self.eps)
+            m = F.silu(self._proj(h, W["mlp.gate_proj.weight"])) * self._proj(h, W["mlp.up_proj.weight"])
+            x = x + self._row_parallel(m, W["mlp.down_proj.weight"])
+        return _rms_norm(x, self.weight("model.norm.weight"), self.eps)
+
+    def _sdpa(self, q, k, v, mask):
+        """[t, nh, hd] queries over [nkv, L, hd] keys where mask [t, L]."""
+        a = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k[None], v[None], attn_mask=mask,
+                                           scale=self.hd ** -0.5, enable_gqa=self.nh != self.nkv)
+        return a[0].transpose(0, 1)
+
+    @torch.no_grad()
+    def forward_packed(self, prompts: list, cache: KVCache) -> torch.Tensor:
+        """One pass over several token sequences of different lengths
+        (1-D int64 tensors), sequence b appended to entry b of `cache`
+        (KVCache(batch=len(prompts))): no padding, every projection one
+        product over all tokens. Returns the logits after each sequence's
+        last token, [len(prompts), vocab]. The fused mode runs the packed
+        kernels of seq_ops; results agree with forward() up to BF16
+        rounding."""
+        if len(prompts) != len(cache.lengths):
+            raise ValueError("forward_packed: %d prompts for a cache of %d sequences" % (len(prompts),
+                                                                                      len(cache.lengths)))
+        lens = [int(p.numel()) for p in prompts]
+        if not lens or min(lens) < 1:
+            raise ValueError("forward_packed: every prompt needs a token")
+        start = list(cache.lengths)
+        ends = [s + m for s, m in zip(start, lens)]
+        if max(ends) > cache.max_len:
+            raise ValueError("forward_packed: %d tokens for a cache of %d" % (max(ends), cache.max_len))
+        cu = [0]
+        for m in lens:
+            cu.append(cu[-1] + m)
+        ids = torch.cat([p.reshape(-1).to(self.device) for p in prompts])
+        self.begin_forward()
+        x = self.embed(ids)
+        if self.fused:
+            from . import seq_ops
+            d_cu = torch.tensor(cu, dtype=torch.int64, device=self.device)
+            len_k = torch.tensor(ends, dtype=torch.int64, device=self.device)
+
+        def attend(i, q):
+            return seq_ops.prompt_attention(q, cache.k[i], cache.v[i], d_cu, self.hd ** -0.5, len_k=len_k)
+
+        def attend_plain(i, q):
+            out = []
+            for b, (s, e) in enumerate(zip(start, ends)):
+                mask = torch.arange(e, device=q.device)[None] <= torch.arange(s, e, device=q.device)[:, None]
+                out.append(self._sdpa(q[cu[b]:cu[b + 1]], cache.k[i][b, :, :e], cache.v[i][b, :, :e], mask))
+            return torch.cat(out)
+
+        x = self._layers_rows(x, cache, cu, start, None, attend, attend_plain)
+        cache.lengths = ends
+        last = torch.tensor([c - 1 for c in cu[1:]], device=x.device)
+        return self._all_gather_last(self.head_logits(x[last]))
+
+    @torch.no_grad()
+    def forward_tree(self, ids: torch.Tensor, mask: torch.Tensor, depth: torch.Tensor, cache: KVCache) -> torch.Tensor:
+        """Logits [T, vocab] of T drafted tokens behind the committed ones
+        of `cache` (one sequence). The last T of the C = mask.shape[1]
+        drafted tokens are given; the C - T before them are in the cache from
+        earlier calls. mask bool [T, C]: which drafted tokens each one sees
+        (itself among them); depth int64 [T]: its distance from the first
+        place behind the committed tokens (seq_ops.tree_mask makes both).
+        Their keys and values stay in the rows behind cache.length, which
+        does not change: keep_drafted commits a path of them."""
+        ids = ids.reshape(-1).to(self.device)
+        T, C = mask.shape
+        pos = cache.length
+        if len(cache.lengths) != 1 or ids.shape[0] != T or depth.shape != (T,) or C < T or T < 1:
+            raise ValueError("forward_tree: a cache of one sequence, T ids and depths and a mask [T, C], C >= T >= 1")
+        if pos + C > cache.max_len:
+            raise ValueError("forward_tree: %d tokens for a cache of %d" % (pos + C, cache.max_len))
+        mask, depth = mask.to(self.device), depth.to(self.device)
+        first = pos + C - T
+        self.begin_forward()
+        x = self.embed(ids)
+        if self.fused:
+            from . import seq_ops
+            d_pos = torch.full((1,), pos, dtype=torch.int64, device=self.device)
+
+        def attend(i, q):
+            return seq_ops.tree_attention(q[None], cache.k[i], cache.v[i], d_pos, mask, self.hd ** -0.5)[0]
+
+        def attend_plain(i, q):
+            seen = torch.cat((torch.ones(T, pos, dtype=torch.bool, device=q.device), mask), 1)
+            return self._sdpa(q, cache.k[i][0, :, :pos + C], cache.v[i][0, :, :pos + C], seen)
+
+        # rotary places count from the first row of this call
+        x = self._layers_rows(x, cache, [0, T], [first], depth - (C - T), attend, attend_plain)
+        return self._all_gather_last(self.head_logits(x))
+
+    def keep_drafted(self, cache: KVCache, path: list) -> None:
+        """Commits the drafted tokens `path` (ascending numbers of a tree
+        given to forward_tree): their keys and values move to the rows right
+        behind the committed ones, in all layers, and count as committed."""
+        if any(b <= a for a, b in zip(path, path[1:])) or (path and path[0] < 0):
+            raise ValueError("keep_drafted: the path's nodes must ascend")
+        if path and cache.length + path[-1] >= cache.max_len:
+            raise ValueError("keep_drafted: node %d lies behind the cache" % path[-1])
+        if list(path) != list(range(len(path))):
+            if self.fused:
+                from . import seq_ops
+                pos = torch.full((1,), cache.length, dtype=torch.int64, device=self.device)
+                keep = torch.tensor([path], dtype=torch.int64, device=self.device)
+                seq_ops.keep_cache_rows(cache.k + cache.v, pos, keep)
+            else:
+                src = torch.tensor(path, device=self.device) + cache.length
+                for c in cache.k + cache.v:
+                    c[:, :, cache.length:cache.length + len(path)] = c[:, :, src]
+        cache.length += len(path)
+
     def embed(self, ids: torch.Tensor) -> torch.Tensor:
         e = self.w["model.embed_tokens.weight"]
         if callable(e):
@@ -753,6 +933,84 @@ class TPDecoder:
             accepted_total += n_draft
         if stats is not None:
             stats.update(sweeps=sweeps, accepted_from_draft=accepted_total, k=k)
+        _device.check_status(self.device)
+        _device.check_status(draft.device)
+        return torch.tensor([committed[:P + max_new_tokens]], device=self.device)
+
+
+    @torch.no_grad()
+    def generate_speculative_tree(self, input_ids: torch.Tensor, max_new_tokens: int, draft: "TPDecoder",
+                                  branch: tuple = (3, 2, 1, 1), stats: dict | None = None) -> torch.Tensor:
+        """Greedy decoding with a drafted tree (generate_speculative drafts a
+        chain): at each level l every node takes the draft's branch[l] most
+        likely tokens as children, and the target scores the pending token
+        and the whole tree in one forward (forward_tree). The path along
+        which each token is the target's own argmax is committed, its cache
+        rows moved together (keep_drafted), and one more token, the target's
+        choice behind the path, is pending. The output is greedy decoding's
+        up to BF16 rounding. Every rank takes the same decisions."""
+        from .seq_ops import tree_mask
+        if draft.vocab != self.vocab:
+            raise ValueError("the draft's vocabulary (%d) does not match the target's (%d)"
+                             % (draft.vocab, self.vocab))
+        branch = tuple(int(b) for b in branch)
+        if not branch or min(branch) < 1 or max(branch) > self.vocab:
+            raise ValueError("branch must name at least one child per level, and no more than there are tokens")
+        ids = input_ids.reshape(1, -1).to(self.device)
+        P = ids.shape[1]
+        if max_new_tokens < 1:
+            return ids
+        # the tree without its root (the pending token): level after level
+        parents, levels = [], []
+        front = [-1]
+        for b in branch:
+            level = []
+            for p in front:
+                for _ in range(b):
+                    level.append(len(parents))
+                    parents.append(p)
+            levels.append(level)
+            front = level
+        d_mask, d_depth = tree_mask(parents, draft.device)
+        t_mask, t_depth = tree_mask([-1] + [p + 1 for p in parents], self.device)
+        children: dict = {}
+        for i, p in enumerate(parents):
+            children.setdefault(p, []).append(i)
+        room = P + max_new_tokens + len(parents) + 2
+        tc = KVCache(self.n_layers, self.nkv, self.hd, room, self.device)
+        dc = KVCache(draft.n_layers, draft.nkv, draft.hd, room, draft.device)
+        first = self.forward_packed([ids[0]], tc)[-1]
+        committed = ids[0].tolist() + [int(first.argmax())]
+        sweeps = accepted = 0
+        while len(committed) - P < max_new_tokens:
+            # draft: what it has not seen of the committed tokens, then a level at a time
+            lg = draft.forward_packed([torch.tensor(committed[dc.length:], device=draft.device)], dc)
+            tokens = torch.zeros(len(parents), dtype=torch.long, device=draft.device)
+            for b, level in zip(branch, levels):
+                tokens[level[0]:level[-1] + 1] = lg.topk(b, -1).indices.reshape(-1)
+                if level is not levels[-1]:
+                    rows = slice(level[0], level[-1] + 1)
+                    lg = draft.forward_tree(tokens[rows], d_mask[rows, :level[-1] + 1], d_depth[rows], dc)
+            # target: the pending token and the tree in one forward
+            pending = torch.tensor([committed[-1]], device=self.device)
+            best = self.forward_tree(torch.cat((pending, tokens.to(self.device))), t_mask, t_depth,
+                                     tc).argmax(-1).tolist()
+            drafted = tokens.tolist()
+            path, new, node = [], [best[0]], -1
+            while True:
+                node = next((c for c in children.get(node, ()) if drafted[c] == new[-1]), None)
+                if node is None:
+                    break
+                path.append(node)
+                new.append(best[node + 1])
+            self.keep_drafted(tc, [0] + [c + 1 for c in path])
+            # the draft has not run the last level
+            draft.keep_drafted(dc, [c for c in path if c < levels[-1][0]])
+            committed += new
+            sweeps += 1
+            accepted += len(path)
+        if stats is not None:
+            stats.update(sweeps=sweeps, accepted_from_draft=accepted, nodes=len(parents))
         _device.check_status(self.device)
         _device.check_status(draft.device)
         return torch.tensor([committed[:P + max_new_tokens]], device=self.device)
