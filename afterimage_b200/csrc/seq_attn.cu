@@ -1001,8 +1001,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (p.splits > 1) {
           if (mine == 0 || !valid) continue;  // (the sum of zero written below says that there is nothing)
+          // four columns of a row side by side, rows next to each other: 512 bytes to a store of the warp
 #pragma unroll
-          for (int i = 0; i < 16; ++i) part[(c + i) * kTile + row] = o[i];
+          for (int i = 0; i < 16; i += 4)
+            reinterpret_cast<float4 *>(part)[(c + i) / 4 * kTile + row] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 16; i += 8)
@@ -1072,10 +1074,22 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   const float *part = p.workspace + (static_cast<int64_t>(item) * p.splits * p.d.nkv * p.tpi + kvh * p.tpi + tile) *
                                         (kTile * (HDP + 2));
   // shares that the item's key tiles do not reach are not read; every other CTA wrote its rows in full
+  const int last = w.shares - 1;
 #pragma unroll 1
-  for (int sp = warp; sp < w.shares; sp += kJoinThreads / 32) {
-    weight[sp][lane] = valid ? part[sp * share + HDP * kTile + row] : -INFINITY;
-    sums[sp][lane] = valid ? part[sp * share + (HDP + 1) * kTile + row] : 0.f;
+  for (int s0 = warp; s0 < w.shares; s0 += kJoinBatch * (kJoinThreads / 32)) {
+    float x[kJoinBatch], y[kJoinBatch];
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b) {
+      const float *r = part + min(s0 + b * (kJoinThreads / 32), last) * share + HDP * kTile + row;
+      x[b] = __ldcg(r);
+      y[b] = __ldcg(r + kTile);
+    }
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b) {
+      const int sp = min(s0 + b * (kJoinThreads / 32), last);
+      weight[sp][lane] = x[b];
+      sums[sp][lane] = y[b];
+    }
   }
   __syncthreads();
   if (!valid || c0 >= p.d.hd) return;
@@ -1084,23 +1098,28 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   for (int sp = 0; sp < w.shares; ++sp) m = fmaxf(m, weight[sp][lane]);
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[8] = {};
-  const float *q = part + c0 * kTile + row;
+  const float4 *q = reinterpret_cast<const float4 *>(part) + c0 / 4 * kTile + row;
 #pragma unroll 1
   for (int s0 = 0; s0 < w.shares; s0 += kJoinBatch) {
-    float x[kJoinBatch][8];
+    float4 x[kJoinBatch][2];
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
-      const float *r = q + min(s0 + b, w.shares - 1) * share;  // behind the last share: again the last, not added
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[b][i] = __ldcg(r + i * kTile);
+      const float4 *r = q + min(s0 + b, last) * (share / 4);  // behind the last share: again the last, times zero
+      x[b][0] = __ldcg(r);
+      x[b][1] = __ldcg(r + kTile);
     }
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
-      if (s0 + b >= w.shares) break;
-      const float a = ex2(weight[s0 + b][lane] - ref);
-      l += a * sums[s0 + b][lane];
+      const int sp = min(s0 + b, last);
+      const float a = s0 + b <= last ? ex2(weight[sp][lane] - ref) : 0.f;
+      l += a * sums[sp][lane];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] += a * x[b][i];
+      for (int i = 0; i < 2; ++i) {
+        o[4 * i] += a * x[b][i].x;
+        o[4 * i + 1] += a * x[b][i].y;
+        o[4 * i + 2] += a * x[b][i].z;
+        o[4 * i + 3] += a * x[b][i].w;
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
