@@ -344,7 +344,8 @@ def keep_cache_rows(caches: list, pos: torch.Tensor, keep: torch.Tensor) -> None
     ptrs = list(map(torch.Tensor.data_ptr, caches))
     # (map: 80 tensors of a 40-layer model are looked at in each call)
     _need(set(map(_dtype_of, caches)) == {_BF16} and set(map(_shape_of, caches)) == {first.shape}
-          and set(map(torch.Tensor.stride, caches)) == {strides} and set(map(torch.Tensor.get_device, caches)) == {dev},
+          and (all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.stride, caches)) == {strides})
+          and set(map(torch.Tensor.get_device, caches)) == {dev},
           f"{who}: caches must be bf16 tensors of one shape, one set of strides and one device")
     _need(strides[3] == 1 or hd == 1, f"{who}: caches need unit stride along the head size")
     _check_not_expanded(who, "a cache", first)
