@@ -984,7 +984,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       static_cast<int64_t>(kvh * p.group) * p.d.out_head_stride;  // the tile's first row
       const uint32_t stage = smem_q + s * C::kSlotBytes + wrow * (2 * HDP);  // 32 rows of HDP values
       const int c_end = second ? (s + 1) * kHalf : HDP;
-#pragma unroll 1
+#pragma unroll 2
       for (int c = second ? s * kHalf : 0; c < c_end; c += 16) {
         float o[16];
         if (mine > 0) {
@@ -1251,6 +1251,8 @@ static int sm_count() {
   return sms;
 }
 
+constexpr int kNoMaps = -1;  // the driver takes no tensor map of this layout: the plain kernel does the call
+
 template <int HDP>
 static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, float *workspace,
                      int32_t *status, cudaStream_t st) {
@@ -1271,7 +1273,7 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
                 1) ||
       !make_map(&mv, d.v, {d.hd, d.key_rows, d.nkv, kb}, {d.v_token_stride, d.v_head_stride, d.v_batch_stride}, kTile,
                 1))
-    return aib_set_errorf("%s: cuTensorMapEncodeTiled failed", who), AIB_ECUDA;
+    return kNoMaps;
   TcParams p;
   p.d = d;
   p.group = pl.group;
@@ -1313,8 +1315,9 @@ static int launch(const aib_attn_desc &d, const char *who, float *workspace, int
     const int64_t need = tc_floats(d, pl);
     if (need && (!workspace || floats < need))
       return aib_set_errorf("%s: needs a workspace of %lld floats", who, (long long)need), AIB_EINVAL;
-    return d.hd <= 64 ? launch_tc<64>(d, tree, pl, who, workspace, status, st)
-                      : launch_tc<128>(d, tree, pl, who, workspace, status, st);
+    const int rc = d.hd <= 64 ? launch_tc<64>(d, tree, pl, who, workspace, status, st)
+                              : launch_tc<128>(d, tree, pl, who, workspace, status, st);
+    if (rc != kNoMaps) return rc;
   }
   const int64_t rows = (tree ? d.batch : 1) * d.tokens * d.nh;
   const int64_t blocks = (rows + kPlainWarps - 1) / kPlainWarps;

@@ -161,6 +161,29 @@ def test_one_key_and_value_for_all_heads_by_an_expanded_tensor():
     R.check(_ops().prompt_attention(q, k, v, _i([0, 90]), 0.1), *R.prompt(q, k, v, _i([0, 90]), 0.1)[:2])
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
+def test_scales_that_are_not_positive(scale):
+    g = _gen(60)
+    q, k, v = _n(g, 150, 4, 128), _n(g, 150, 2, 128), _n(g, 150, 2, 128)
+    R.check(_ops().prompt_attention(q, k, v, _cu([100, 50]), scale), *R.prompt(q, k, v, _cu([100, 50]), scale)[:2])
+
+
+def test_no_keys_at_all():
+    q, k = torch.ones(5, 4, 64, dtype=BF, device=DEV), torch.ones(0, 2, 64, dtype=BF, device=DEV)
+    out = torch.full_like(q, 3.0)
+    _ops().prompt_attention(q, k, k, _cu([2, 3]), 0.1, cu_k=_cu([0, 0]), out=out)
+    assert not out.any()
+
+
+def test_the_output_may_be_the_queries():
+    """A block has read its queries before it writes them, also where the key axis is shared out."""
+    g = _gen(61)
+    for n, nh, nkv in ((700, 4, 2), (300, 160, 32)):
+        q, k, v = _n(g, n, nh, 128), _n(g, n, nkv, 128), _n(g, n, nkv, 128)
+        want = _ops().prompt_attention(q, k, v, _cu([n - 30, 30]), 0.1)
+        assert torch.equal(_ops().prompt_attention(q, k, v, _cu([n - 30, 30]), 0.1, out=q), want)
+
+
 def test_large_scores():
     """Scores of several hundred, rising along the keys: the running maximum has to follow, and early weights vanish."""
     g = _gen(7)
