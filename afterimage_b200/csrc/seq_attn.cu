@@ -984,8 +984,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                       static_cast<int64_t>(kvh * p.group) * p.d.out_head_stride;  // the tile's first row
       const uint32_t stage = smem_q + s * C::kSlotBytes + wrow * (2 * HDP);  // 32 rows of HDP values
       const int c_end = second ? (s + 1) * kHalf : HDP;
-#pragma unroll 2
-      for (int c = second ? s * kHalf : 0; c < c_end; c += 16) {
+      int c = second ? s * kHalf : 0;
+      if (!second && p.splits == 1 && mine > 0) {  // the whole row at once
+        uint32_t o[HDP];
+#pragma unroll
+        for (int i = 0; i < HDP; i += 32) tmem_ld32(to + i, o + i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < HDP; i += 8) {
+          uint32_t x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            x[k] = pack_bf16(__uint_as_float(o[i + 2 * k]) * a0, __uint_as_float(o[i + 2 * k + 1]) * a0);
+          sts128(stage + lane * (2 * HDP) + (((i / 8) ^ (lane & 7)) * 16), make_uint4(x[0], x[1], x[2], x[3]));
+        }
+        c = c_end;
+      }
+#pragma unroll 1
+      for (; c < c_end; c += 16) {
         float o[16];
         if (mine > 0) {
           tmem_ld16(to + c, reinterpret_cast<uint32_t *>(o));
@@ -1018,21 +1034,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         // part of the Q tile (nothing reads it any more) a row's 16-byte pieces go out together.
         __syncwarp();
         const int per = second ? kHalf / 8 : HDP / 8;  // pieces of a row; a power of two
-        const int first = second ? s * per : 0;
+        const int at_once = 32 / per;                  // rows that the warp writes in one go
+        const int q = (second ? s * per : 0) + lane % per;
+        int r = lane / per;
+        int head = wrow + r - ((wrow + r) * p.group_rcp >> 16) * p.group;
+        uint16_t *to_row = out + static_cast<int64_t>((wrow + r) * p.group_rcp >> 16) * p.d.out_token_stride +
+                           head * p.d.out_head_stride + q * 8;
+        const int64_t next_token = p.d.out_token_stride - p.group * p.d.out_head_stride;
+        if (q * 8 < p.d.hd) {
 #pragma unroll 4
-        for (int e = lane; e < 32 * per; e += 32) {
-          const int r = e / per, q = first + e % per;
-          if (wrow + r >= rows || q * 8 >= p.d.hd) continue;
-          const int to_tok = ((wrow + r) * p.group_rcp) >> 16;
-          uint16_t *to_row = out + to_tok * p.d.out_token_stride +
-                             static_cast<int64_t>(wrow + r - to_tok * p.group) * p.d.out_head_stride + q * 8;
-          uint32_t x[4];
-          lds128(stage + r * (2 * HDP) + ((q ^ (r & 7)) * 16), x);
-          if (p.vec_out) {
-            *reinterpret_cast<uint4 *>(to_row) = make_uint4(x[0], x[1], x[2], x[3]);
-          } else {
+          for (; r < 32 && wrow + r < rows; r += at_once) {
+            uint32_t x[4];
+            lds128(stage + r * (2 * HDP) + ((q ^ (r & 7)) * 16), x);
+            if (p.vec_out) {
+              *reinterpret_cast<uint4 *>(to_row) = make_uint4(x[0], x[1], x[2], x[3]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to_row[i] = static_cast<uint16_t>(x[i / 2] >> (16 * (i & 1)));
+              for (int i = 0; i < 8; ++i) to_row[i] = static_cast<uint16_t>(x[i / 2] >> (16 * (i & 1)));
+            }
+            to_row += at_once * p.d.out_head_stride;
+            for (head += at_once; head >= p.group; head -= p.group) to_row += next_token;
           }
         }
       }
