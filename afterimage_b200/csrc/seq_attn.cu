@@ -20,6 +20,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "aib_internal.h"
 
@@ -858,20 +859,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.f;
     const int mine = pair ? (s ? nk : n0) : (nk + 1 - s) / 2;
     bool ok = true;
-    for (int it = 0; it < mine; ++it) {
+    // one tile; a copy of its own for the tiles that every row sees in full (all but the last few of a long prompt)
+    const auto softmax_tile = [&](int it, auto masked) {
+      constexpr bool kMasked = decltype(masked)::value;
       const int j = pair ? it : 2 * it + s;
       const int t = w.ta + j;
-      const bool masked = (t + 1) * kTile > low;
       uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      if (masked && active) seen_words(p, w.s, t0, tok, tok0, tok1, t, bits);
-      if (!(ok = warp_wait(smem_u32(&bar_s[s]), it & 1, &gave_up))) break;
+      if (kMasked && active) seen_words(p, w.s, t0, tok, tok0, tok1, t, bits);
+      if (!warp_wait(smem_u32(&bar_s[s]), it & 1, &gave_up)) return false;
       fence_after();
       if (active) {
         uint32_t x[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, x + 32 * c);
         tmem_wait_ld();
-        if (masked) {
+        if (kMasked) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (!((bits[i / 32] >> (i % 32)) & 1u)) x[i] = 0xff800000u;  // -infinity
@@ -932,7 +934,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_p[s][1]));
-    }
+      return true;
+    };
+    int it = 0;
+    const int full = max(0, min(mine, pair ? low / kTile - w.ta : (low / kTile - w.ta - s + 1) / 2));
+#pragma unroll 1
+    for (; ok && it < full; ++it) ok = softmax_tile(it, std::false_type{});
+#pragma unroll 1
+    for (; ok && it < mine; ++it) ok = softmax_tile(it, std::true_type{});
     if (ok && mine > 0) ok = warp_wait(smem_u32(&bar_o[s]), 0, &gave_up);
     fence_after();
 
