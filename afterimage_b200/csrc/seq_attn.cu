@@ -198,6 +198,28 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
 // some row is added back, row by row, at the end.
 // Every wait is bounded; one that gives up sets AIB_STATUS_WAIT_TIMEOUT and
 // the CTA unwinds.
+//
+// What bounds it. For a pair, 128 keys are 32 matrix instructions of 64 clocks
+// each (2048 clocks) and 256 exponentials a scheduler at 8 clocks each (2048
+// clocks); the two would have to overlap in full, and tensor memory has no room
+// for a second S beside two O of 128 columns, so that a stream's next scores
+// wait for its product with V. Measured: about 3700 clocks, tensor pipe and
+// exponential unit both busy 47 %. One prompt of 16384 tokens, 40 heads of 128
+// on 8 kv heads, causal: 2.21 ms in a burst (1240 TFLOP/s, 0.75 of the measured
+// cuBLAS burst), 2.7 ms in a loop of seconds (0.71-0.73 of cuBLAS in such a
+// loop), where the power limit holds the clock at 1.67 GHz.
+// What was tried and did not pay there: exponentials by a polynomial on the
+// multiply-add pipe for 1/8 to 3/8 of the weights (2.27 -> 2.27, 2.31 and 2.37
+// ms); S in halves of 64 keys, the two in turn (2.41 ms: a product with 64
+// columns reads Q as often as one with 128); a sixth ring tile, and prefetches
+// into L2, where there is one Q tile (no change).
+// A drafted tree of 64 nodes over 32,000 slots (three tiles a kv head, six
+// shares): 60 us, of which the join is 5; the keys and values are read from
+// HBM once (133 MB by the counters, 2.4 TB/s) and from L2 three times.
+// Short calls are a chain of waits: set-up 1 us, first tiles 1.5, a tile's
+// scores, softmax and product 2, the output 1, and where the key axis is shared
+// out 1.4 until the join starts and 2-3 for it. One token over 1000 slots: 11.5
+// us; a chain of five over 4099: 16 us.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 128;
 constexpr int kThreads = 384;
@@ -942,7 +964,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (; ok && it < full; ++it) ok = softmax_tile(it, std::false_type{});
 #pragma unroll 1
     for (; ok && it < mine; ++it) ok = softmax_tile(it, std::true_type{});
-    if (ok && mine > 0) ok = warp_wait(smem_u32(&bar_o[s]), 0, &gave_up);
+    // a stream without tiles has no products to wait for; its Q tile, which its rows go out through, still has to land
+    if (ok && (mine > 0 || nk > 0)) ok = warp_wait(mine > 0 ? smem_u32(&bar_o[s]) : smem_u32(&bar_q), 0, &gave_up);
     fence_after();
 
     if (mine > 0 && active && ok && __any_sync(0xffffffffu, *static_cast<volatile int *>(&bad_seen) != 0)) {
@@ -1257,7 +1280,11 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
   pl.tpi = 2;
   pl.splits = 1;
   pl.items = item_bound(d, tree, 2LL * pl.tt);
-  // two tiles over the same keys halve the loads, but only where that still gives every SM an item
+  // Two tiles over the same keys halve the loads, but only where that still gives every SM an item. Where it does
+  // not, one tile a CTA and a share of the key axis. 64 nodes over 32,000 slots: 497 us with two tiles and no shares,
+  // 253 us with one tile and none, 86 us with two and nine shares, 63 us with one and six; 317 queries of two prompts
+  // over 8000 and 4100 keys, one kv head: 134, 77, 31 and 28 us. Sixteen sequences of 26 nodes fill 128 of 148 SMs
+  // and are not shared out: 36 us, with two, three and four shares each 37, 40 and 43 us.
   if (pl.items * d.nkv < sms) {
     pl.tpi = 1;
     pl.items = item_bound(d, tree, pl.tt);

@@ -102,6 +102,18 @@ def test_queries_before_their_first_key_are_zero():
     assert not got[:153].any() and not got[290:297].any()
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(148, 148, 128), (148, 74, 64)])
+def test_a_first_tile_that_sees_nothing_beside_a_second_that_does(nh, nkv, hd):
+    g = _gen(62)
+    for m, L in ((600, 200), (512, 130), (300, 44)):
+        q, k, v = _n(g, m, nh, hd), _n(g, L, nkv, hd), _n(g, L, nkv, hd)
+        for _ in range(4):
+            out = torch.full_like(q, 5.0)
+            _ops().prompt_attention(q, k, v, _cu([m]), 0.1, cu_k=_cu([L]), out=out)
+            assert not out[:m - L].any()
+        R.check(out, *R.prompt(q, k, v, _cu([m]), 0.1, cu_k=_cu([L]))[:2])
+
+
 def test_rows_outside_every_sequence_stay():
     g = _gen(2)
     q, k, v = _n(g, 200, 8, 128), _n(g, 200, 2, 128), _n(g, 200, 2, 128)
