@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import array
 import ctypes
-import operator
 import struct
 
 import torch
@@ -323,7 +322,28 @@ def rope_cache_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, cu: torch.T
     return out
 
 
-_shape_of, _dtype_of = operator.attrgetter("shape"), operator.attrgetter("dtype")
+_shape_of, _dtype_of = torch.Tensor.shape.__get__, torch.Tensor.dtype.__get__
+
+
+def _all_are(values, value, n: int) -> bool:
+    return list(values).count(value) == n
+
+
+def _check_keep(caches, pos, keep, ptrs) -> None:
+    who = "keep_cache_rows"
+    first = caches[0]
+    _check_device(who, first, pos, keep)
+    _need(first.dim() == 4, f"{who}: caches must be [B, kv heads, max_len, head size]")
+    for t in caches:
+        _need(t.dtype == _BF16 and t.shape == first.shape and t.stride() == first.stride() and t.device == first.device,
+              f"{who}: caches must be bf16 tensors of one shape, one set of strides and one device")
+    _need(first.stride(3) == 1 or first.shape[3] == 1, f"{who}: caches need unit stride along the head size")
+    _check_not_expanded(who, "a cache", first)
+    _need(first.numel() == 0 or len(set(ptrs)) == len(ptrs), f"{who}: a cache is given twice")
+    _need(keep.dim() == 2, f"{who}: keep must be int64 [B, n]")
+    _need(keep.shape[1] <= MAX_KEEP, f"{who}: {keep.shape[1]} rows, at most {MAX_KEEP}")
+    _check_index(who, (first.shape[0],), pos=pos)
+    _check_index(who, (first.shape[0], keep.shape[1]), keep=keep)
 
 
 def keep_cache_rows(caches: list, pos: torch.Tensor, keep: torch.Tensor) -> None:
@@ -333,37 +353,33 @@ def keep_cache_rows(caches: list, pos: torch.Tensor, keep: torch.Tensor) -> None
     pos[b] + i <- row pos[b] + keep[b, i] as it was before the call, for the
     n <= 256 columns of keep (int64 [B, n]). keep < 0, and rows outside the
     cache, leave the row as it is. The caches must not overlap."""
-    who = "keep_cache_rows"
     if not caches:
         return
     first = caches[0]
-    _check_device(who, first, pos, keep)
-    _need(first.dim() == 4, f"{who}: caches must be [B, kv heads, max_len, head size]")
-    b, nkv, max_len, hd = first.shape
-    strides, dev = first.stride(), first.get_device()
+    shape, strides, dev = first.shape, first.stride(), first.get_device()
+    n = len(caches)
     ptrs = list(map(torch.Tensor.data_ptr, caches))
-    # (map: 80 tensors of a 40-layer model are looked at in each call)
-    _need(set(map(_dtype_of, caches)) == {_BF16} and set(map(_shape_of, caches)) == {first.shape}
-          and (all(map(torch.Tensor.is_contiguous, caches)) or set(map(torch.Tensor.stride, caches)) == {strides})
-          and set(map(torch.Tensor.get_device, caches)) == {dev},
-          f"{who}: caches must be bf16 tensors of one shape, one set of strides and one device")
-    _need(strides[3] == 1 or hd == 1, f"{who}: caches need unit stride along the head size")
-    _check_not_expanded(who, "a cache", first)
-    _need(first.numel() == 0 or len(set(ptrs)) == len(ptrs), f"{who}: a cache is given twice")
-    _need(keep.dim() == 2, f"{who}: keep must be int64 [B, n]")
-    n = keep.shape[1]
-    _need(n <= MAX_KEEP, f"{who}: {n} rows, at most {MAX_KEEP}")
-    _check_index(who, (b,), pos=pos)
-    _check_index(who, (b, n), keep=keep)
-    _check_cuda(who, first)
+    # (map over the type's own accessors: 80 tensors of a 40-layer model are looked at in each call)
+    usual = (len(shape) == 4 and _all_are(map(_dtype_of, caches), _BF16, n)
+             and _all_are(map(_shape_of, caches), shape, n)
+             and (_all_are(map(torch.Tensor.is_contiguous, caches), True, n)
+                  or _all_are(map(torch.Tensor.stride, caches), strides, n))
+             and _all_are(map(torch.Tensor.get_device, caches), dev, n) and len(set(ptrs)) == n and dev >= 0
+             and strides[3] == 1 and min(strides) > 0 and pos.dtype is _I64 and keep.dtype is _I64
+             and pos.get_device() == dev and keep.get_device() == dev and pos.shape == shape[:1] and keep.dim() == 2
+             and keep.shape[0] == shape[0] and keep.shape[1] <= MAX_KEEP and pos.is_contiguous()
+             and keep.is_contiguous())
+    if not usual:
+        _check_keep(caches, pos, keep, ptrs)
+        _check_cuda("keep_cache_rows", first)
     if first.numel() == 0:
         return
 
     def call():
         table = array.array("Q", ptrs)
-        return _lib.load().aib_keep_cache_rows_bf16(table.buffer_info()[0], len(ptrs), b, nkv, max_len, hd,
+        return _lib.load().aib_keep_cache_rows_bf16(table.buffer_info()[0], n, *shape,
                                                     struct.pack("3q", *strides[:3]), pos.data_ptr(), keep.data_ptr(),
-                                                    n, _raw_stream(dev))
+                                                    keep.shape[1], _raw_stream(dev))
 
     if torch._C._cuda_getDevice() == dev:
         rc = call()
@@ -371,7 +387,7 @@ def keep_cache_rows(caches: list, pos: torch.Tensor, keep: torch.Tensor) -> None
         with torch.cuda.device(dev):
             rc = call()
     if rc:
-        _lib.check(rc, who)
+        _lib.check(rc, "keep_cache_rows")
 
 
 def tree_mask(parents, device=None) -> tuple[torch.Tensor, torch.Tensor]:
