@@ -538,6 +538,15 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 x) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 
+// What the warps of a CTA share of its item, in shared memory; read where it is needed, so that it takes no registers
+// beside a tile of scores.
+enum Field { kLive, kQ0, kQb, kKb, kK0, kKeys, kOff, kT0, kCnt0, kCnt1, kEnd, kLow0, kLow1, kTa, kPairs, kTiles, kTiles0, kSeenInFull, kFields };
+__device__ __forceinline__ int lds32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // bits of the seen keys among the four 32-key words of key tile t, for this
 // thread's row (token tok of the tile; first token of the tile is ti within
 // the sequence). Collective over the warp for trees.
@@ -612,6 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2][2], bar_o[2], bar_drain, bar_dirty, bar_clean;
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up, bad_seen;
+  __shared__ int fields[kFields];
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // (all kv heads of the largest item first: with the items of one head after the other the mixed prompts took a
@@ -649,17 +659,50 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
   }
-  const Item w = make_item(p, item, split);
-
-  const bool pair = w.live && w.cnt1 > 0;
-  // pair: key tiles of each stream (the second tile's tokens are later: they see as many or more);
-  // solo: the tiles that both streams take in turn
-  const int n0 = !w.live ? 0 : max(0, min((w.end0 + kTile - 1) / kTile, w.tb) - w.ta);
-  const int nk = !w.live ? 0 : pair ? max(n0, min((w.end1 + kTile - 1) / kTile, w.tb) - w.ta) : n0;
-  // the first key tile of this share that some row does not see in full
-  const int first_masked = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
-
-  const int pairs = uniform(pair), n_k = uniform(nk), n_0 = uniform(n0), n_full = uniform(first_masked);
+  const auto field = [&](int f) { return lds32(smem_u32(&fields[f])); };
+  int pairs, n_k, k_row = 0, k_b = 0;
+  if (warp == 8) {
+    // looks up what the CTA works on and asks for the first tiles; the others take it from there (all twelve warps
+    // looking it up took each other's issue slots)
+    const Item w = make_item(p, item, split);
+    const bool pair = w.live && w.cnt1 > 0;
+    // pair: key tiles of each stream (the second tile's tokens are later: they see as many or more);
+    // solo: the tiles that both streams take in turn
+    const int n0 = !w.live ? 0 : max(0, min((w.end0 + kTile - 1) / kTile, w.tb) - w.ta);
+    const int nk = !w.live ? 0 : pair ? max(n0, min((w.end1 + kTile - 1) / kTile, w.tb) - w.ta) : n0;
+    if (elect()) {
+      fields[kLive] = w.live;
+      fields[kQ0] = w.s.q0;
+      fields[kQb] = w.s.qb;
+      fields[kKb] = w.s.kb;
+      fields[kK0] = w.s.k0;
+      fields[kKeys] = w.s.L;
+      fields[kOff] = w.s.off;
+      fields[kT0] = w.t0;
+      fields[kCnt0] = w.cnt0;
+      fields[kCnt1] = w.cnt1;
+      fields[kEnd] = max(w.end0, w.end1);
+      fields[kLow0] = w.low0;
+      fields[kLow1] = w.low1;
+      fields[kTa] = w.ta;
+      fields[kPairs] = pair;
+      fields[kTiles] = nk;
+      fields[kTiles0] = n0;
+      // the first key tile of this share that some row does not see in full
+      fields[kSeenInFull] = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
+    }
+    __syncwarp();
+    asm volatile("bar.arrive 2, 384;" ::: "memory");
+    pairs = uniform(pair);
+    n_k = uniform(nk);
+    k_row = uniform(w.s.k0 + w.ta * kTile);
+    k_b = uniform(w.s.kb);
+  } else {
+    asm volatile("bar.sync 2, 384;" ::: "memory");
+    fence_after();
+    pairs = uniform(field(kPairs));
+    n_k = uniform(field(kTiles));
+  }
   // The ring holds the tiles in the order in which the matrix instructions want them: K0 V0 K1 V1 ... for a pair,
   // K0 K1 V0 K2 V1 ... solo.
   const auto pos_v = [&](int j) { return pairs ? 2 * j + 1 : (j == n_k - 1 ? 2 * n_k - 1 : 2 * j + 2); };
@@ -670,7 +713,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     return is_v;
   };
   const int early = min(2 * n_k, C::kSlots);  // tiles that fit the empty ring: asked for before anything else
-  const int k_row = uniform(w.s.k0 + w.ta * kTile), k_b = uniform(w.s.kb);
   const auto fetch = [&](const CUtensorMap *map, int j, int slot) {
     if (elect()) {
       const uint32_t fb = smem_u32(&bar_full[slot]);
@@ -682,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   };
   if (warp == 8 && n_k > 0) {
-    const int q_row = uniform(w.s.q0 + w.t0), q_b = uniform(w.s.qb);
+    const int q_row = uniform(field(kQ0) + field(kT0)), q_b = uniform(field(kQb));
     if (elect()) {
       const uint32_t qbar = smem_u32(&bar_q);
       const uint32_t bytes = static_cast<uint32_t>(p.group * p.tt * 128 * C::kHalves);
@@ -700,8 +742,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       fetch(is_v ? &map_v : &map_k, j, pos);
     }
   }
-  __syncthreads();
-  fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the whole tensor memory is taken, so it starts at column 0: S (and P) of stream s at 128 s, O at 256 + 128 s
 
@@ -738,6 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t id_s = idesc_bf16(kTile, 0), id_o = idesc_bf16(HDP, 1);
         const uint32_t dq = desc_kmajor(smem_q), dk = desc_kmajor(ring), dv = desc_mnmajor(ring);
         constexpr uint32_t kSlotStep = C::kSlotBytes >> 4;
+        const int n_0 = uniform(field(kTiles0)), n_full = uniform(field(kSeenInFull));
         unsigned clean_ph = 0, p_ph = 0, open = 0;  // p_ph, open: a bit per stream; open: its O has been written
         int slot = 0, k = 0, v = 0;
         unsigned phase = 0;
@@ -826,12 +867,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       // ---- V tiles that some row does not see in full: what is not finite becomes zero
-      const int seen_end = max(w.end0, w.end1);
+      const int seen_end = field(kEnd), ta = field(kTa), first_masked = field(kSeenInFull);
       const int self = static_cast<int>(threadIdx.x) - 320;
-      for (int j = first_masked; j < nk; ++j) {
+      for (int j = first_masked; j < n_k; ++j) {
         if (!warp_wait(smem_u32(&bar_dirty), (j - first_masked) & 1u, &gave_up)) break;
         const uint32_t base = ring + (pos_v(j) % C::kSlots) * C::kSlotBytes;
-        const int rows_seen = seen_end - (w.ta + j) * kTile;
+        const int rows_seen = seen_end - (ta + j) * kTile;
         // a value times zero is zero unless it is not finite: one multiply-add for two values finds whether any is
         const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
         __nv_bfloat162 any = zero;
@@ -863,13 +904,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(smem_u32(&bar_clean));
       }
     }
-  } else if (w.live) {  // uniform over the CTA
+  } else if (field(kLive)) {  // uniform over the CTA
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax: one thread per row of the stream's tile
     const int s = warp >> 2;
-    const int tile = pair ? s : 0;
-    const int cnt = tile ? w.cnt1 : w.cnt0, low = tile ? w.low1 : w.low0;
-    const int t0 = w.t0 + tile * p.tt;  // first token of the tile
+    const bool pair = pairs;
+    const int nk = n_k, tile = pair ? s : 0;
+    const int cnt = field(tile ? kCnt1 : kCnt0);
     const int wrow = (warp & 3) * 32, row = wrow + lane;
     const int rows = cnt * p.group;
     const bool active = wrow < rows;  // a warp without rows only keeps the barriers going
@@ -879,15 +920,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = s * 128 + lanes, to = 256 + s * 128 + lanes;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
-    const int mine = pair ? (s ? nk : n0) : (nk + 1 - s) / 2;
+    const int mine = pair ? (s ? nk : field(kTiles0)) : (nk + 1 - s) / 2;
     bool ok = true;
+    const auto seq = [&] {
+      Seq r;
+      r.q0 = field(kQ0), r.m = 0, r.qb = field(kQb), r.kb = field(kKb), r.k0 = field(kK0), r.L = field(kKeys);
+      r.off = field(kOff);
+      return r;
+    };
     // one tile; a copy of its own for the tiles that every row sees in full (all but the last few of a long prompt)
     const auto softmax_tile = [&](int it, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
-      const int j = pair ? it : 2 * it + s;
-      const int t = w.ta + j;
       uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      if (kMasked && active) seen_words(p, w.s, t0, tok, tok0, tok1, t, bits);
+      if (kMasked && active)
+        seen_words(p, seq(), field(kT0) + tile * p.tt, tok, tok0, tok1, field(kTa) + (pair ? it : 2 * it + s), bits);
       if (!warp_wait(smem_u32(&bar_s[s]), it & 1, &gave_up)) return false;
       fence_after();
       if (active) {
@@ -959,7 +1005,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
     int it = 0;
-    const int full = max(0, min(mine, pair ? low / kTile - w.ta : (low / kTile - w.ta - s + 1) / 2));
+    const int in_full = field(tile ? kLow1 : kLow0) / kTile - field(kTa);
+    const int full = max(0, min(mine, pair ? in_full : (in_full - s + 1) / 2));
 #pragma unroll 1
     for (; ok && it < full; ++it) ok = softmax_tile(it, std::false_type{});
 #pragma unroll 1
@@ -969,10 +1016,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after();
 
     if (mine > 0 && active && ok && __any_sync(0xffffffffu, *static_cast<volatile int *>(&bad_seen) != 0)) {
-      const int step = pair ? 1 : 2;
+      const int step = pair ? 1 : 2, first_masked = field(kSeenInFull), ta = field(kTa);
       int first = pair ? 0 : s;
       if (first < first_masked) first += (first_masked - first + step - 1) / step * step;
-      add_not_finite<HDP>(p, w.s, t0, kvh, tok, tok0, tok1, w.ta + first, w.ta + (pair ? mine : nk), step, to);
+      add_not_finite<HDP>(p, seq(), field(kT0) + tile * p.tt, kvh, tok, tok0, tok1, ta + first,
+                          ta + (pair ? mine : nk), step, to);
     }
     // Solo: the two streams' sums over the same rows are joined through shared memory (over the ring, whose last tile
     // both have waited for): each stream hands over the half of its columns that the other one finishes.
@@ -1011,8 +1059,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       a1 *= inv;
       const int64_t unit = ((static_cast<int64_t>(item) * p.splits + split) * p.d.nkv + kvh) * p.tpi + tile;
       float *part = p.workspace + unit * (kTile * (HDP + 2));
-      uint16_t *out = static_cast<uint16_t *>(p.d.out) + w.s.qb * p.d.out_batch_stride +
-                      static_cast<int64_t>(w.s.q0 + t0) * p.d.out_token_stride +
+      uint16_t *out = static_cast<uint16_t *>(p.d.out) + field(kQb) * p.d.out_batch_stride +
+                      static_cast<int64_t>(field(kQ0) + field(kT0) + tile * p.tt) * p.d.out_token_stride +
                       static_cast<int64_t>(kvh * p.group) * p.d.out_head_stride;  // the tile's first row
       const uint32_t stage = smem_q + s * C::kSlotBytes + wrow * (2 * HDP);  // 32 rows of HDP values
       const int c_end = second ? (s + 1) * kHalf : HDP;
