@@ -958,7 +958,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float a = m == -INFINITY ? 0.f : ex2(m - mn);
           if (it > 0) {
             // the stream's previous P V is done: its S was ready only after it
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HDP / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(to + 32 * c, o);
