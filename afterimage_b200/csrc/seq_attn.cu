@@ -203,23 +203,22 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
 // each (2048 clocks) and 256 exponentials a scheduler at 8 clocks each (2048
 // clocks); the two would have to overlap in full, and tensor memory has no room
 // for a second S beside two O of 128 columns, so that a stream's next scores
-// wait for its product with V. Measured: about 3700 clocks, tensor pipe and
-// exponential unit both busy 47 %. One prompt of 16384 tokens, 40 heads of 128
-// on 8 kv heads, causal: 2.21 ms in a burst (1240 TFLOP/s, 0.75 of the measured
-// cuBLAS burst), 2.7 ms in a loop of seconds (0.71-0.73 of cuBLAS in such a
-// loop), where the power limit holds the clock at 1.67 GHz.
+// wait for its product with V. Measured: about 3600 clocks, tensor pipe and
+// exponential unit both busy half of the time. One prompt of 16384 tokens, 40
+// heads of 128 on 8 kv heads, causal: 2.15 ms in a burst (1280 TFLOP/s, 0.77 of
+// the measured cuBLAS burst), 2.65 ms in a loop of seconds (1040, 0.75 of cuBLAS
+// in such a loop), where the power limit holds the clock at 1.67 GHz.
 // What was tried and did not pay there: exponentials by a polynomial on the
-// multiply-add pipe for 1/8 to 3/8 of the weights (2.27 -> 2.27, 2.31 and 2.37
-// ms); S in halves of 64 keys, the two in turn (2.41 ms: a product with 64
-// columns reads Q as often as one with 128); a sixth ring tile, and prefetches
-// into L2, where there is one Q tile (no change).
+// multiply-add pipe for 1/8 or 2/8 of the weights (2.14 -> 2.16 and 2.19 ms); S
+// in halves of 64 keys, the two in turn (2.41 against 2.31 ms then: a product
+// with 64 columns reads Q as often as one with 128); a sixth ring tile, and
+// prefetches into L2, where there is one Q tile (no change).
 // A drafted tree of 64 nodes over 32,000 slots (three tiles a kv head, six
-// shares): 60 us, of which the join is 5; the keys and values are read from
-// HBM once (133 MB by the counters, 2.4 TB/s) and from L2 three times.
+// shares): 53 us, of which the join is 5; the keys and values are read from
+// HBM once (133 MB by the counters, 2.5 TB/s) and from L2 three times.
 // Short calls are a chain of waits: set-up 1 us, first tiles 1.5, a tile's
-// scores, softmax and product 2, the output 1, and where the key axis is shared
-// out 1.4 until the join starts and 2-3 for it. One token over 1000 slots: 11.5
-// us; a chain of five over 4099: 16 us.
+// scores, softmax and product 2, the output 1, joining the shares 1 to 4. One
+// token over 1000 slots: 9.4 us; a chain of five over 4099: 13.1 us.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 128;
 constexpr int kThreads = 384;
@@ -241,6 +240,7 @@ struct TcParams {
   int group_rcp;       // r / group is r * group_rcp >> 16 for r < 128
   int tpi;             // tiles an item may hold: 2 or 1
   int splits;          // shares of the key axis
+  int cluster;         // the shares are one cluster's CTAs and join through its shared memory, without a second kernel
   int items;           // upper bound of the items
   float scale_log2;
   int vec_out;         // output rows allow 16-byte stores
@@ -415,8 +415,9 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 // with the descriptors built for each instruction it was what the 16384-token
 // prompt waited for.)
 constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return addr >> 4 | 1u << 16; }
-__device__ __forceinline__ uint32_t desc_mnmajor(uint32_t addr) { return addr >> 4 | (16384u >> 4) << 16; }
+// (in a cluster the high bits of a shared address say whose memory it is)
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4 & 0x3fff) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mnmajor(uint32_t addr) { return (addr >> 4 & 0x3fff) | (16384u >> 4) << 16; }
 
 // BF16 x BF16 -> F32, M = 128
 __host__ __device__ constexpr uint32_t idesc_bf16(int n, int b_mn_major) {
@@ -526,6 +527,28 @@ __device__ __forceinline__ float max_nan3(float a, float b, float c) {
   return d;
 }
 
+// shared memory of another CTA of the cluster: the address there of what is at `addr` here
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ bool not_finite_bf16(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
 
 __device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&x)[4]) {
@@ -540,7 +563,7 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 x) {
 
 // What the warps of a CTA share of its item, in shared memory; read where it is needed, so that it takes no registers
 // beside a tile of scores.
-enum Field { kLive, kQ0, kQb, kKb, kK0, kKeys, kOff, kT0, kCnt0, kCnt1, kEnd, kLow0, kLow1, kTa, kPairs, kTiles, kTiles0, kSeenInFull, kFields };
+enum Field { kLive, kQ0, kQb, kKb, kK0, kKeys, kOff, kT0, kCnt0, kCnt1, kEnd, kLow0, kLow1, kTa, kPairs, kTiles, kTiles0, kSeenInFull, kShares, kFields };
 __device__ __forceinline__ int lds32(uint32_t addr) {
   int v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -609,6 +632,49 @@ __device__ __forceinline__ void add_not_finite(const TcParams &p, const Seq &s, 
     tmem_st1(to + c, o);
   }
   tmem_wait_st();
+}
+
+// Joins a cluster's shares: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, each CTA for HDP / shares columns,
+// two threads to a row. `part`: where each CTA has its share's O (four columns of a row side by side), maxima and
+// sums.
+template <int HDP, typename F>
+__device__ __forceinline__ void join_cluster(const TcParams &p, uint32_t part, int kvh, int rank, const F &field) {
+  const int row = threadIdx.x & (kTile - 1);
+  if (row >= field(kCnt0) * p.group) return;
+  const int shares = min(p.splits, field(kShares));
+  const int width = HDP / p.splits / 2;  // columns of a thread: 4 (16 shares) to 32 (2)
+  const int c0 = rank * (HDP / p.splits) + static_cast<int>(threadIdx.x >> 7) * width;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int s = 0; s < shares; ++s) m = fmaxf(m, ld_cluster(in_cta(part, s) + (HDP * kTile + row) * 4));
+  const float ref = m == -INFINITY ? 0.f : m;
+  const int tok = (row * p.group_rcp) >> 16;
+  uint16_t *out = static_cast<uint16_t *>(p.d.out) + field(kQb) * p.d.out_batch_stride +
+                  static_cast<int64_t>(field(kQ0) + field(kT0) + tok) * p.d.out_token_stride +
+                  static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
+#pragma unroll 1
+  for (int c = c0; c < c0 + width && c < p.d.hd; c += 4) {
+    float l = 0.f, o[4] = {};
+#pragma unroll 4
+    for (int s = 0; s < shares; ++s) {
+      const uint32_t at = in_cta(part, s);
+      const float a = ex2(ld_cluster(at + (HDP * kTile + row) * 4) - ref);
+      const float4 x = ld_cluster4(at + (c / 4 * kTile + row) * 16);
+      l += a * ld_cluster(at + ((HDP + 1) * kTile + row) * 4);
+      o[0] += a * x.x;
+      o[1] += a * x.y;
+      o[2] += a * x.z;
+      o[3] += a * x.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t lo = pack_bf16(o[0] * inv, o[1] * inv), hi = pack_bf16(o[2] * inv, o[3] * inv);
+    if (p.vec_out) {
+      *reinterpret_cast<uint2 *>(out + c) = make_uint2(lo, hi);
+    } else {
+      out[c] = static_cast<uint16_t>(lo), out[c + 1] = static_cast<uint16_t>(lo >> 16);
+      out[c + 2] = static_cast<uint16_t>(hi), out[c + 3] = static_cast<uint16_t>(hi >> 16);
+    }
+  }
 }
 
 template <int HDP>
@@ -688,6 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fields[kPairs] = pair;
       fields[kTiles] = nk;
       fields[kTiles0] = n0;
+      fields[kShares] = w.live ? w.shares : 0;
       // the first key tile of this share that some row does not see in full
       fields[kSeenInFull] = max(0, (pair ? min(w.low0, w.low1) : w.low0) / kTile - w.ta);
     }
@@ -1058,7 +1125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       a0 *= inv;
       a1 *= inv;
       const int64_t unit = ((static_cast<int64_t>(item) * p.splits + split) * p.d.nkv + kvh) * p.tpi + tile;
-      float *part = p.workspace + unit * (kTile * (HDP + 2));
+      float *part = p.cluster ? joined + (HDP + 4) * kTile : p.workspace + unit * (kTile * (HDP + 2));
       uint16_t *out = static_cast<uint16_t *>(p.d.out) + field(kQb) * p.d.out_batch_stride +
                       static_cast<int64_t>(field(kQ0) + field(kT0) + tile * p.tt) * p.d.out_token_stride +
                       static_cast<int64_t>(kvh * p.group) * p.d.out_head_stride;  // the tile's first row
@@ -1143,6 +1210,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     fence_before();
+  }
+  __syncwarp();
+  if (p.cluster) {
+    cluster_barrier();  // every share's rows are in its CTA's shared memory
+    if (warp < 8 && field(kLive)) join_cluster<HDP>(p, ring + (HDP + 4) * kTile * 4, kvh, split, field);
+    __syncwarp();
+    cluster_barrier();  // and none leaves while another one reads it
   }
   __syncthreads();
   if (threadIdx.x == 0 && gave_up && p.status) atomicOr(p.status, AIB_STATUS_WAIT_TIMEOUT);
@@ -1312,8 +1386,12 @@ static bool tensor_cores(const aib_attn_desc &d, bool tree) {
 
 struct TcPlan {
   int group, tt, tpi, splits;
+  bool cluster;
   int64_t items;
 };
+
+// clusters of `shares` CTAs of the attention kernel that the current device holds at once (0: none, or not known)
+static int clusters_at_once(int hd, int shares);
 
 static int64_t item_bound(const aib_attn_desc &d, bool tree, int64_t unit) {
   if (tree) return d.batch * ((d.tokens + unit - 1) / unit);
@@ -1327,6 +1405,7 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
   pl.tt = kTile / pl.group;
   pl.tpi = 2;
   pl.splits = 1;
+  pl.cluster = false;
   pl.items = item_bound(d, tree, 2LL * pl.tt);
   // Two tiles over the same keys halve the loads, but only where that still gives every SM an item. Where it does
   // not, one tile a CTA and a share of the key axis. 64 nodes over 32,000 slots: 497 us with two tiles and no shares,
@@ -1339,13 +1418,31 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
     const int64_t units = std::max<int64_t>(1, pl.items * d.nkv);
     // shares of at least two key tiles (one for each stream), at most one CTA per SM
     const int64_t tiles = (d.key_rows + kTile - 1) / kTile;
-    pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / units, (tiles + 1) / 2), kMaxSplits)));
+    const int64_t cap = std::max<int64_t>(1, sms / units);
+    pl.splits = static_cast<int>(std::min<int64_t>(std::min<int64_t>(cap, (tiles + 1) / 2), kMaxSplits));
+    // Shares that are one cluster join in its shared memory and need no second kernel and no workspace. A cluster has
+    // 2, 4, 8 or 16 CTAs of one GPC, so there are fewer shares; taken where that costs at most three more rounds of two
+    // key tiles, which is what the second kernel costs (a round is 1.2 us, its start and its work 3 to 4). One token
+    // over 1000 slots: 9.4 us, against 10.9 with a second kernel; a chain of five over 4099 (8 shares, against 18):
+    // 13.1 and 15.2; 317 queries over 8000 and 4100 keys (8, against 10): 19.9 and 22.4; but 64 nodes over 32,000 slots
+    // (4, against 6): 68 and 53.
+    if (pl.splits > 1) {
+      int s = 2;
+      while (s < pl.splits && s < 16) s *= 2;
+      if (s > cap) s /= 2;
+      while (s > 1 && clusters_at_once(d.hd, s) < units) s /= 2;  // all at once, or the last ones wait for the first
+      const auto rounds = [&](int64_t shares) { return ((tiles + shares - 1) / shares + 1) / 2; };
+      if (s > 1 && rounds(s) <= rounds(pl.splits) + 3) {
+        pl.splits = s;
+        pl.cluster = true;
+      }
+    }
   }
   return pl;
 }
 
 static int64_t tc_floats(const aib_attn_desc &d, const TcPlan &pl) {
-  if (pl.splits == 1) return 0;
+  if (pl.splits == 1 || pl.cluster) return 0;
   const int hdp = d.hd <= 64 ? 64 : 128;
   return pl.items * pl.splits * d.nkv * pl.tpi * kTile * (hdp + 2);
 }
@@ -1356,19 +1453,65 @@ static int sm_count() {
   return sms;
 }
 
-constexpr int kNoMaps = -1;  // the driver takes no tensor map of this layout: the plain kernel does the call
-
+// once per device: the shared-memory limit, and clusters of 16
 template <int HDP>
-static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, float *workspace,
-                     int32_t *status, cudaStream_t st) {
-  // the shared-memory limit is set once per device
+static cudaError_t prepare_kernel() {
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(ready.load() >> dev & 1))) {
     e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HDP>::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
+  return e;
+}
+
+static cudaLaunchAttribute cluster_of(int shares) {
+  cudaLaunchAttribute a;
+  a.id = cudaLaunchAttributeClusterDimension;
+  a.val.clusterDim.x = 1;
+  a.val.clusterDim.y = static_cast<unsigned>(shares);
+  a.val.clusterDim.z = 1;
+  return a;
+}
+
+template <int HDP>
+static int query_clusters(int shares) {
+  if (prepare_kernel<HDP>() != cudaSuccess) return (void)cudaGetLastError(), 0;
+  cudaLaunchAttribute a = cluster_of(shares);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1, static_cast<unsigned>(shares));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<HDP>::kSmem;
+  cfg.attrs = &a;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, attn_tc_kernel<HDP>, &cfg) != cudaSuccess) return (void)cudaGetLastError(), 0;
+  return n;
+}
+
+static int clusters_at_once(int hd, int shares) {
+  static std::atomic<int> known[64][2][17];  // 0: not asked yet; n + 1 otherwise
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return (void)cudaGetLastError(), 0;
+  const bool wide = hd > 64;
+  if (dev < 64) {
+    const int k = known[dev][wide][shares].load();
+    if (k) return k - 1;
+  }
+  const int n = wide ? query_clusters<128>(shares) : query_clusters<64>(shares);
+  if (dev < 64) known[dev][wide][shares].store(n + 1);
+  return n;
+}
+
+constexpr int kNoMaps = -1;  // the driver takes no tensor map of this layout: the plain kernel does the call
+
+template <int HDP>
+static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, float *workspace,
+                     int32_t *status, cudaStream_t st) {
+  cudaError_t e = prepare_kernel<HDP>();
   if (e != cudaSuccess) return aib_set_errorf("%s: %s", who, cudaGetErrorString(e)), AIB_ECUDA;
   const int64_t kb = tree || d.len_k ? d.batch : 1;
   CUtensorMap mq, mk, mv;
@@ -1386,6 +1529,7 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   p.tt = pl.tt;
   p.tpi = pl.tpi;
   p.splits = pl.splits;
+  p.cluster = pl.cluster;
   p.items = static_cast<int>(pl.items);
   p.scale_log2 = d.scale * 1.4426950408889634f;
   p.vec_out = aligned16(d.out) && d.out_token_stride % 8 == 0 && d.out_head_stride % 8 == 0 &&
@@ -1393,17 +1537,22 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   p.workspace = workspace;
   p.status = status;
   const dim3 grid(static_cast<unsigned>(pl.items * d.nkv), static_cast<unsigned>(pl.splits));
-  attn_tc_kernel<HDP><<<grid, kThreads, Cfg<HDP>::kSmem, st>>>(mq, mk, mv, p);
-  if ((e = cudaGetLastError()) == cudaSuccess && pl.splits > 1) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = cluster_of(pl.splits);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<HDP>::kSmem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = pl.cluster ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, attn_tc_kernel<HDP>, mq, mk, mv, p);
+  if (e == cudaSuccess && pl.splits > 1 && !pl.cluster) {
     // started while the last shares still run (it waits for them before it reads)
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(pl.items), static_cast<unsigned>(d.nkv), 4 * pl.tpi * (HDP / 32));
     cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = st;
-    cfg.attrs = &early;
+    cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, attn_join_kernel<HDP>, p);
   }
