@@ -102,6 +102,7 @@ class AttnDesc(ctypes.Structure):
         ("cu_q", P), ("cu_k", P), ("len_k", P), ("pos", P), ("mask", P),
         ("mask_batch_stride", I64), ("mask_row_stride", I64), ("mask_col_stride", I64),
         ("mask_cols", I64),
+        ("sms", I64),
     ]
 
 

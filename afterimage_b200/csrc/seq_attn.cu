@@ -1327,6 +1327,7 @@ static int check_common(const aib_attn_desc *p, const char *who) {
   const int64_t big = INT32_MAX - 1024;  // room for a tile behind the last row
   if (p->tokens > big || p->batch > big || p->key_rows > big)
     return aib_set_errorf("%s: tokens, batch and key rows must fit in 32 bits (below 2^31 - 1024)", who), AIB_EINVAL;
+  if (p->sms < 0) return aib_set_errorf("%s: sms is negative", who), AIB_EINVAL;
   if (!std::isfinite(p->scale)) return aib_set_errorf("%s: scale is not finite", who), AIB_EINVAL;
   return AIB_OK;
 }
@@ -1399,7 +1400,8 @@ static int64_t item_bound(const aib_attn_desc &d, bool tree, int64_t unit) {
   return std::min(d.tokens, (d.tokens + d.batch * (unit - 1)) / unit);
 }
 
-static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
+static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int device_sms) {
+  const int sms = d.sms > 0 ? static_cast<int>(std::min<int64_t>(d.sms, device_sms)) : device_sms;
   TcPlan pl;
   pl.group = d.nh / d.nkv;
   pl.tt = kTile / pl.group;
@@ -1432,7 +1434,7 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int sms) {
       if (s > cap) s /= 2;
       while (s > 1 && clusters_at_once(d.hd, s) < units) s /= 2;  // all at once, or the last ones wait for the first
       const auto rounds = [&](int64_t shares) { return ((tiles + shares - 1) / shares + 1) / 2; };
-      if (s > 1 && rounds(s) <= rounds(pl.splits) + 3) {
+      if (d.sms == 0 && s > 1 && rounds(s) <= rounds(pl.splits) + 3) {
         pl.splits = s;
         pl.cluster = true;
       }

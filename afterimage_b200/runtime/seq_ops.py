@@ -29,9 +29,9 @@ _F32 = torch.float32
 MAX_HEAD_SIZE = 256
 MAX_KEEP = 256
 
-# aib_attn_desc, packed in one go: a step makes two calls a layer, and setting 36 ctypes fields one by one takes
+# aib_attn_desc, packed in one go: a step makes two calls a layer, and setting 37 ctypes fields one by one takes
 # longer than the kernel of a short tree
-_DESC = struct.Struct("@4P15q3if5P4q")
+_DESC = struct.Struct("@4P15q3if5P5q")
 assert _DESC.size == ctypes.sizeof(_lib.AttnDesc)
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -134,7 +134,7 @@ def _check_prompt(q, k, v, cu_q, cu_k, len_k, out) -> None:
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, scale: float, *,
                      cu_k: torch.Tensor | None = None, len_k: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, sms: int = 0) -> torch.Tensor:
     """Causal attention of packed prompts: q [N, nh, hd], cu_q [B + 1].
 
     Keys are packed too (k, v [Nk, nkv, hd], cu_k [B + 1], default cu_q), or
@@ -142,7 +142,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     prompt's own among them). A sequence's queries are the last of its keys:
     row i of m sees the keys j <= L - m + i. Rows that see nothing are zero;
     rows of q in no sequence are not computed and their rows of `out` not
-    written. Returns out [N, nh, hd] (new unless given)."""
+    written. Returns out [N, nh, hd] (new unless given; it may be q). `sms`:
+    how many SMs the call may count on while kernels of other streams hold
+    the rest (0: all of them)."""
     shape, kshape = q.shape, k.shape
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     dev = q.get_device()
@@ -173,7 +175,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     os = out.stride()
     _call("aib_prompt_attention_bf16", "prompt_attention", q, _DESC.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, qs[0], qs[1], *strides, 0, os[0], os[1],
-        n, cu_q.shape[0] - 1, rows, nh, nkv, hd, scale, cu_q.data_ptr(), starts, lens, 0, 0, 0, 0, 0, 0))
+        n, cu_q.shape[0] - 1, rows, nh, nkv, hd, scale, cu_q.data_ptr(), starts, lens, 0, 0, 0, 0, 0, 0, sms))
     return out
 
 
@@ -198,7 +200,7 @@ def _check_tree(q, k_cache, v_cache, pos, mask, out) -> None:
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor,
-                   mask: torch.Tensor, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+                   mask: torch.Tensor, scale: float, out: torch.Tensor | None = None, sms: int = 0) -> torch.Tensor:
     """Attention of T drafted tokens per sequence over its cache: q
     [B, T, nh, hd], caches [B, nkv, max_len, hd], pos int64 [B].
 
@@ -206,7 +208,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     tokens are at the slots pos[b] .. pos[b] + C - 1, and query i sees those
     with mask[i, j] (mask bool [T, C] for all sequences or [B, T, C]; see
     tree_mask). T = C = 1 is the single-token step of a batch. A query that
-    sees nothing gives zeros. Returns [B, T, nh, hd] (new unless given)."""
+    sees nothing gives zeros. Returns [B, T, nh, hd] (new unless given; it
+    may be q). `sms`: as for prompt_attention."""
     shape, kshape, mshape = q.shape, k_cache.shape, mask.shape
     qs, ks, vs, ms = q.stride(), k_cache.stride(), v_cache.stride(), mask.stride()
     dev = q.get_device()
@@ -229,7 +232,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _call("aib_tree_attention_bf16", "tree_attention", q, _DESC.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), *qs[:3], *ks[:3], *vs[:3],
         *out.stride()[:3], t, b, kshape[2], nh, kshape[1], hd, scale, 0, 0, 0, at, mask.data_ptr() or at,
-        ms[0] if len(ms) == 3 else 0, ms[-2], ms[-1], mshape[-1]))
+        ms[0] if len(ms) == 3 else 0, ms[-2], ms[-1], mshape[-1], sms))
     return out
 
 

@@ -282,6 +282,7 @@ class TPDecoder:
         self.timeline = None  # a list to record (kind, layer, start event, end event) into
         self._graph_state = None
         self.allreducer = None  # one-shot NVLink all-reduce (use_oneshot_allreduce); else NCCL
+        self.free_sms = 0       # SMs that the layer math may count on (0: all); fewer beside an overlapped decode
         rp = getattr(hf_cfg, "rope_parameters", None) or {}
         theta = rp.get("rope_theta", getattr(hf_cfg, "rope_theta", 10000.0))
         self.inv_freq = 1.0 / (theta ** (torch.arange(0, self.hd, 2, dtype=torch.int64).to(
@@ -614,7 +615,8 @@ class TPDecoder:
             len_k = torch.tensor(ends, dtype=torch.int64, device=self.device)
 
         def attend(i, q):
-            return seq_ops.prompt_attention(q, cache.k[i], cache.v[i], d_cu, self.hd ** -0.5, len_k=len_k)
+            return seq_ops.prompt_attention(q, cache.k[i], cache.v[i], d_cu, self.hd ** -0.5, len_k=len_k,
+                                            sms=self.free_sms)
 
         def attend_plain(i, q):
             out = []
@@ -654,7 +656,8 @@ class TPDecoder:
             d_pos = torch.full((1,), pos, dtype=torch.int64, device=self.device)
 
         def attend(i, q):
-            return seq_ops.tree_attention(q[None], cache.k[i], cache.v[i], d_pos, mask, self.hd ** -0.5)[0]
+            return seq_ops.tree_attention(q[None], cache.k[i], cache.v[i], d_pos, mask, self.hd ** -0.5,
+                                          sms=self.free_sms)[0]
 
         def attend_plain(i, q):
             seen = torch.cat((torch.ones(T, pos, dtype=torch.bool, device=q.device), mask), 1)
@@ -1170,6 +1173,8 @@ class CompressedTPDecoder(TPDecoder):
         if decode_sms is None:
             decode_sms = round(0.78 * torch.cuda.get_device_properties(self.dev).multi_processor_count)
         self.decode_sms = int(decode_sms) if self.overlap else 0
+        if self.decode_sms > 0:
+            self.free_sms = max(1, torch.cuda.get_device_properties(self.dev).multi_processor_count - self.decode_sms)
         self._ahead: dict = {}
         # decoded weights land in preallocated output sets (two when the decode of layer
         # i+1 overlaps layer i's projections), so descriptors are built once per

@@ -196,6 +196,18 @@ def test_the_output_may_be_the_queries():
         assert torch.equal(_ops().prompt_attention(q, k, v, _cu([n - 30, 30]), 0.1, out=q), want)
 
 
+@pytest.mark.parametrize("sms", [1, 20, 33, 100, 1000])
+def test_beside_other_kernels(sms):
+    """Fewer SMs to count on: other shares and no clusters, the same result up to the order of sums."""
+    g = _gen(63)
+    q, k, v = _n(g, 1, 5, 32, 128), _n(g, 1, 8, 3000, 128), _n(g, 1, 8, 3000, 128)
+    mask, _ = _ops().tree_mask([-1, 0, 1, 1, 0], DEV)
+    R.check(_ops().tree_attention(q, k, v, _i([2900]), mask, 0.1, sms=sms), *R.tree(q, k, v, [2900], mask, 0.1))
+    q, k, v = _n(g, 700, 10, 64), _n(g, 700, 5, 64), _n(g, 700, 5, 64)
+    R.check(_ops().prompt_attention(q, k, v, _cu([600, 100]), 0.1, sms=sms),
+            *R.prompt(q, k, v, _cu([600, 100]), 0.1)[:2])
+
+
 def test_large_scores():
     """Scores of several hundred, rising along the keys: the running maximum has to follow, and early weights vanish."""
     g = _gen(7)

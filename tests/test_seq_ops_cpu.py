@@ -166,7 +166,7 @@ def _desc(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(nh=3), b"shape"), (dict(nkv=0), b"shape"), (dict(hd=257), b"shape"), (dict(tokens=-1), b"shape"),
     (dict(tokens=2 ** 31), b"32 bits"), (dict(scale=float("nan")), b"scale"), (dict(q=None), b"null"),
-    (dict(v=None), b"null"), (dict(out=None), b"null"),
+    (dict(v=None), b"null"), (dict(out=None), b"null"), (dict(sms=-1), b"sms"),
 ])
 def test_attention_c_entries_refuse(entry, kw, text):
     L = _lib.load()
