@@ -36,6 +36,9 @@ def attend(q, k, v, seen, scale):
     for j in torch.nonzero(bad).flatten().tolist():
         rows = seen[:, j]
         out[rows] += p[rows, j:j + 1] * v[j]
+        # its finite values count in sum p |v| like all others: without them the sum can lie below |out|, which it bounds
+        # (one seen key of weight 0.9 and value 0.35 beside a NaN: |out| 0.35, the sum without it 0.03)
+        size[rows] += p[rows, j:j + 1] * torch.where(torch.isfinite(v[j]), v[j].abs(), 0.0)
     return out, size
 
 
