@@ -179,13 +179,13 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
 // makes one pass over a kv head's keys serve all its queries. A CTA takes two
 // tiles of consecutive tokens over the same keys ("pair"), or one tile whose
 // key tiles two streams take in turn and join at the end ("solo"), and,
-// where that would leave SMs empty, a share of the key axis; the shares are
-// joined by a second kernel.
+// where that would leave SMs empty, a share of the key axis; the shares join
+// through a cluster's shared memory or in a second kernel.
 //
 // Per CTA, 128 keys at a time:
 //   S = Q K^T         tcgen05.mma, both operands in shared memory -> tensor memory
 //   P = exp2(S - m)   one thread per row: running maximum and sum, P as BF16
-//                     over S's columns in tensor memory
+//                     over S's columns in tensor memory, or beside them
 //   O = O + P V       tcgen05.mma, P from tensor memory, V as it lies in
 //                     shared memory (keys x head size)
 // The running maximum is only followed when it would leave P above 2^8: any
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
 // each (2048 clocks) and 256 exponentials a scheduler at 8 clocks each (2048
 // clocks); the two would have to overlap in full, and tensor memory has no room
 // for a second S beside two O of 128 columns, so that a stream's next scores
-// wait for its product with V. Measured: about 3600 clocks, tensor pipe and
+// wait for its product with V (64 columns leave the room). Measured: about 3600 clocks, tensor pipe and
 // exponential unit both busy half of the time. One prompt of 16384 tokens, 40
 // heads of 128 on 8 kv heads, causal: 2.15 ms in a burst (1280 TFLOP/s, 0.77 of
 // the measured cuBLAS burst), 2.65 ms in a loop of seconds (1040, 0.75 of cuBLAS
@@ -226,12 +226,20 @@ constexpr int kMaxSlots = 8;
 constexpr unsigned kWaitLimit = AIB_WAIT_LIMIT_POLLS;
 constexpr float kFollow = 8.f;  // log2 of how far above 1 a weight may come before the maximum is followed
 
-template <int HDP>
+template <int HDP, bool kOwnP>
 struct Cfg {
   static constexpr int kHalves = HDP / 64;             // 128-byte-swizzled column blocks of a tile
   static constexpr int kSlotBytes = kHalves * 16384;   // one K, V or Q tile
   static constexpr int kSlots = HDP == 128 ? 5 : 8;
   static constexpr int kSmem = (2 + kSlots) * kSlotBytes + 1024;
+  // With O of 64 columns P can have columns of its own (kOwnP): a stream's next scores are made as soon as the last
+  // ones are in registers, and the softmax does not wait for them, for one more signal and wait a tile. With O of 128
+  // P lies over S, and the scores wait for its product. Two tiles on the same keys gain by it, one tile does not: 8192
+  // tokens, 32 heads of 64 on 8: 401 -> 373 us, seven prompts of 1 to 3000: 121 -> 115, 32 trees of 49 nodes: 53 -> 51;
+  // 64 trees of 8: 79 -> 81, 317 queries over 8000 and 4100 keys: 55.5 -> 59.4. So items of two tiles have it.
+  static_assert(!kOwnP || HDP == 64);
+  static constexpr int kColO = 256, kColP = 384;  // tensor-memory columns; S of stream s at 128 s
+  static constexpr int kStepO = kOwnP ? 64 : 128, kStepP = kOwnP ? 64 : 128;
 };
 
 struct TcParams {
@@ -677,14 +685,15 @@ __device__ __forceinline__ void join_cluster(const TcParams &p, uint32_t part, i
   }
 }
 
-template <int HDP>
+template <int HDP, bool kOwnP>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
-  using C = Cfg<HDP>;
+  using C = Cfg<HDP, kOwnP>;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t bar_full[kMaxSlots], bar_empty[kMaxSlots];
-  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2][2], bar_o[2], bar_drain, bar_dirty, bar_clean;
+  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_taken[2], bar_p[2][2], bar_pv[2];
+  __shared__ __align__(8) uint64_t bar_drain, bar_dirty, bar_clean;
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up, bad_seen;
   __shared__ int fields[kFields];
@@ -706,7 +715,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&bar_s[s]), 1);
       mbar_init(smem_u32(&bar_p[s][0]), 4);
       mbar_init(smem_u32(&bar_p[s][1]), 4);
-      mbar_init(smem_u32(&bar_o[s]), 1);
+      mbar_init(smem_u32(&bar_taken[s]), 4);
+      mbar_init(smem_u32(&bar_pv[s]), 1);
     }
     mbar_init(smem_u32(&bar_drain), 1);
     mbar_init(smem_u32(&bar_dirty), 1);
@@ -770,14 +780,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     pairs = uniform(field(kPairs));
     n_k = uniform(field(kTiles));
   }
-  // The ring holds the tiles in the order in which the matrix instructions want them: K0 V0 K1 V1 ... for a pair,
-  // K0 K1 V0 K2 V1 ... solo.
-  const auto pos_v = [&](int j) { return pairs ? 2 * j + 1 : (j == n_k - 1 ? 2 * n_k - 1 : 2 * j + 2); };
+  // The ring holds the tiles in the order in which the matrix instructions want them: `ahead` K tiles, then the next K
+  // and a V in turn, then the V that are left.
+  const int ahead = (pairs ? 0 : 1) + (kOwnP ? 1 : 0);
+  const auto pos_v = [&](int j) { return j + ahead < n_k ? ahead + 2 * j + 1 : n_k + j; };
   const auto at = [&](int pos, int &j) {  // what is at a ring position: tile number, and whether it is V's
-    const bool end = pos == 2 * n_k - 1, odd = pos & 1;
-    const bool is_v = pairs ? odd : (pos > 0 && (!odd || end));
-    j = pairs ? pos >> 1 : (end ? n_k - 1 : (is_v ? pos / 2 - 1 : (pos + 1) / 2));
-    return is_v;
+    if (pos < min(ahead, n_k)) {
+      j = pos;
+      return false;
+    }
+    const int q = max(0, pos - ahead);
+    if (q / 2 + ahead < n_k) {
+      j = q / 2 + (q & 1 ? 0 : ahead);
+      return (q & 1) != 0;
+    }
+    j = pos - n_k;
+    return true;
   };
   const int early = min(2 * n_k, C::kSlots);  // tiles that fit the empty ring: asked for before anything else
   const auto fetch = [&](const CUtensorMap *map, int j, int slot) {
@@ -810,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // the whole tensor memory is taken, so it starts at column 0: S (and P) of stream s at 128 s, O at 256 + 128 s
+  // the whole tensor memory is taken, so it starts at column 0 (Cfg has what lies where)
 
   // 384 threads start with 168 registers each; the softmax warps take over what the others leave
   // (256 x 216 + 128 x 72 = 384 x 168)
@@ -857,15 +875,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++slot == C::kSlots) slot = 0, phase ^= 1u;
           return r;
         };
-        // Step u: the product with V of key tile j, then the scores of that stream's next tile. A pair's streams
-        // share key tile j = u div 2; solo, tile j = u belongs to stream j mod 2. The first two steps only make scores.
+        // Step u: the product with V of key tile j and the scores of that stream's next tile js; the scores first where
+        // they need not wait for the product. A pair's streams share key tile j = u div 2; solo, tile j = u belongs to
+        // stream j mod 2. The first two steps only make scores.
         const int total = pairs ? 2 * n_k : n_k;
+        unsigned taken_ph = 0;
+        const auto scores = [&](const int s, int js, int mine, bool takes, bool leaves) {
+          if (js >= n_k) return true;
+          if (takes && !next(k)) return false;
+          if (js < mine) {
+            fence_after();
+            if (elect()) {
+              const uint32_t a = dq + (pairs ? s * kSlotStep : 0), b = dk + k * kSlotStep;
+#pragma unroll
+              for (int i = 0; i < C::kHalves * 4; ++i)
+                mma_ss(s * 128, a + (i / 4) * 1024 + (i % 4) * 2, b + (i / 4) * 1024 + (i % 4) * 2, id_s, i > 0);
+              mma_commit(smem_u32(&bar_s[s]));
+              if (leaves) mma_commit(smem_u32(&bar_empty[k]));
+            }
+            __syncwarp();
+          }
+          return true;
+        };
         // (two steps to an iteration: the streams' addresses are constants then)
         const auto step = [&](const int u, const int s) {
           const int j = pairs ? u >> 1 : u, js = pairs ? j + 1 : j + 2;
           const int mine = pairs && s == 0 ? n_0 : n_k;  // this stream's tiles lie before this one
           const bool takes = !pairs || s == 0, leaves = !pairs || s == 1;
-          const uint32_t ts = s * 128, to = 256 + s * 128;
+          const uint32_t ts = (kOwnP ? C::kColP : 0) + s * C::kStepP, to = C::kColO + s * C::kStepO;
+          if (kOwnP) {
+            if (j >= 0 && js < mine) {
+              if (!warp_wait(smem_u32(&bar_taken[s]), taken_ph >> s & 1u, &gave_up)) return false;
+              taken_ph ^= 1u << s;
+            }
+            if (!scores(s, js, mine, takes, leaves)) return false;
+          }
           if (j >= 0) {
             if (takes) {
               if (!next(v)) return false;
@@ -896,27 +940,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int i = kTile / 32; i < kTile / 16; ++i) mma_ts(to, ts + i * 8, b + i * 128, id_o, 1);
                 if (leaves) mma_commit(smem_u32(&bar_empty[v]));
-                if (js >= mine) mma_commit(smem_u32(&bar_o[s]));
+                if (kOwnP || js >= mine) mma_commit(smem_u32(&bar_pv[s]));
               }
               __syncwarp();
             }
           }
-          if (js < n_k) {
-            if (takes && !next(k)) return false;
-            if (js < mine) {
-              fence_after();
-              if (elect()) {
-                const uint32_t a = dq + (pairs ? s * kSlotStep : 0), b = dk + k * kSlotStep;
-#pragma unroll
-                for (int i = 0; i < C::kHalves * 4; ++i)
-                  mma_ss(ts, a + (i / 4) * 1024 + (i % 4) * 2, b + (i / 4) * 1024 + (i % 4) * 2, id_s, i > 0);
-                mma_commit(smem_u32(&bar_s[s]));
-                if (leaves) mma_commit(smem_u32(&bar_empty[k]));
-              }
-              __syncwarp();
-            }
-          }
-          return true;
+          return kOwnP || scores(s, js, mine, takes, leaves);
         };
 #pragma unroll 1
         for (int u = -2; ok && u < total; u += 2) {
@@ -984,7 +1013,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tok = min((row * p.group_rcp) >> 16, cnt - 1);
     const int tok0 = (wrow * p.group_rcp) >> 16, tok1 = min(((wrow + 31) * p.group_rcp) >> 16, cnt - 1);
     const uint32_t lanes = static_cast<uint32_t>(wrow) << 16;
-    const uint32_t ts = s * 128 + lanes, to = 256 + s * 128 + lanes;
+    const uint32_t ts = s * 128 + lanes, to = C::kColO + s * C::kStepO + lanes;
+    const uint32_t tp = (kOwnP ? C::kColP : 0) + s * C::kStepP + lanes;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.f;
     const int mine = pair ? (s ? nk : field(kTiles0)) : (nk + 1 - s) / 2;
@@ -1008,6 +1038,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, x + 32 * c);
         tmem_wait_ld();
+        if (kOwnP) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_taken[s]));
+        }
         if (kMasked) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -1020,11 +1055,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           top[i / 2 % 4] = max_nan3(top[i / 2 % 4], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
         const float mz = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * sl;
         const bool follow = !(mz <= m + kFollow);
+        // P and O are free once the product of the stream's previous tile is done (where P lies over S, this tile's
+        // scores were ready only after it)
+        if (kOwnP && it > 0) {
+          if (!warp_wait(smem_u32(&bar_pv[s]), (it - 1) & 1, &gave_up)) return false;
+          fence_after();
+        }
         if (__any_sync(0xffffffffu, follow)) {
           const float mn = follow ? mz : m;
           const float a = m == -INFINITY ? 0.f : ex2(m - mn);
           if (it > 0) {
-            // the stream's previous P V is done: its S was ready only after it
 #pragma unroll 1
             for (int c = 0; c < HDP / 32; ++c) {
               uint32_t o[32];
@@ -1052,7 +1092,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum[i % 2] = add2(sum[i % 2], two(__float_as_uint(e0), __float_as_uint(e1)));
             pk[i] = pack_bf16(e0, e1);  // the matrix product takes BF16; the sum keeps fp32
           }
-          tmem_st16(ts + 16 * c, pk);
+          tmem_st16(tp + 16 * c, pk);
           if (c == 1) {  // the first 64 keys' weights can be used
             tmem_wait_st();
             fence_before();
@@ -1063,8 +1103,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t both = add2(sum[0], sum[1]);
         l += low_of(both) + high_of(both);
         tmem_wait_st();
-      } else if (lane == 0) {
-        mbar_arrive(smem_u32(&bar_p[s][0]));
+      } else {
+        if (kOwnP) {
+          if (lane == 0) mbar_arrive(smem_u32(&bar_taken[s]));
+          // no further than the warps with rows: an arrival counts for the phase that is open
+          if (it > 0 && !warp_wait(smem_u32(&bar_pv[s]), (it - 1) & 1, &gave_up)) return false;
+        }
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p[s][0]));
       }
       fence_before();
       __syncwarp();
@@ -1079,7 +1124,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
     for (; ok && it < mine; ++it) ok = softmax_tile(it, std::true_type{});
     // a stream without tiles has no products to wait for; its Q tile, which its rows go out through, still has to land
-    if (ok && (mine > 0 || nk > 0)) ok = warp_wait(mine > 0 ? smem_u32(&bar_o[s]) : smem_u32(&bar_q), 0, &gave_up);
+    if (ok && mine > 0) ok = warp_wait(smem_u32(&bar_pv[s]), kOwnP ? (mine - 1) & 1 : 0, &gave_up);
+    if (ok && mine == 0 && nk > 0) ok = warp_wait(smem_u32(&bar_q), 0, &gave_up);
     fence_after();
 
     if (mine > 0 && active && ok && __any_sync(0xffffffffu, *static_cast<volatile int *>(&bad_seen) != 0)) {
@@ -1405,7 +1451,7 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int device_sms) {
   TcPlan pl;
   pl.group = d.nh / d.nkv;
   pl.tt = kTile / pl.group;
-  pl.tpi = 2;
+  pl.tpi = tree && d.tokens <= pl.tt ? 1 : 2;
   pl.splits = 1;
   pl.cluster = false;
   pl.items = item_bound(d, tree, 2LL * pl.tt);
@@ -1456,15 +1502,15 @@ static int sm_count() {
 }
 
 // once per device: the shared-memory limit, and clusters of 16
-template <int HDP>
+template <int HDP, bool kOwnP>
 static cudaError_t prepare_kernel() {
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(ready.load() >> dev & 1))) {
-    e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HDP>::kSmem);
+    e = cudaFuncSetAttribute(attn_tc_kernel<HDP, kOwnP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HDP, kOwnP>::kSmem);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      e = cudaFuncSetAttribute(attn_tc_kernel<HDP, kOwnP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
   }
   return e;
@@ -1481,16 +1527,16 @@ static cudaLaunchAttribute cluster_of(int shares) {
 
 template <int HDP>
 static int query_clusters(int shares) {
-  if (prepare_kernel<HDP>() != cudaSuccess) return (void)cudaGetLastError(), 0;
+  if (prepare_kernel<HDP, false>() != cudaSuccess) return (void)cudaGetLastError(), 0;
   cudaLaunchAttribute a = cluster_of(shares);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1, static_cast<unsigned>(shares));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<HDP>::kSmem;
+  cfg.dynamicSmemBytes = Cfg<HDP, false>::kSmem;
   cfg.attrs = &a;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, attn_tc_kernel<HDP>, &cfg) != cudaSuccess) return (void)cudaGetLastError(), 0;
+  if (cudaOccupancyMaxActiveClusters(&n, attn_tc_kernel<HDP, false>, &cfg) != cudaSuccess) return (void)cudaGetLastError(), 0;
   return n;
 }
 
@@ -1510,10 +1556,10 @@ static int clusters_at_once(int hd, int shares) {
 
 constexpr int kNoMaps = -1;  // the driver takes no tensor map of this layout: the plain kernel does the call
 
-template <int HDP>
+template <int HDP, bool kOwnP>
 static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const char *who, float *workspace,
                      int32_t *status, cudaStream_t st) {
-  cudaError_t e = prepare_kernel<HDP>();
+  cudaError_t e = prepare_kernel<HDP, kOwnP>();
   if (e != cudaSuccess) return aib_set_errorf("%s: %s", who, cudaGetErrorString(e)), AIB_ECUDA;
   const int64_t kb = tree || d.len_k ? d.batch : 1;
   CUtensorMap mq, mk, mv;
@@ -1543,11 +1589,11 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   cudaLaunchAttribute attr = cluster_of(pl.splits);
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<HDP>::kSmem;
+  cfg.dynamicSmemBytes = Cfg<HDP, kOwnP>::kSmem;
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = pl.cluster ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, attn_tc_kernel<HDP>, mq, mk, mv, p);
+  e = cudaLaunchKernelEx(&cfg, attn_tc_kernel<HDP, kOwnP>, mq, mk, mv, p);
   if (e == cudaSuccess && pl.splits > 1 && !pl.cluster) {
     // started while the last shares still run (it waits for them before it reads)
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1571,8 +1617,10 @@ static int launch(const aib_attn_desc &d, const char *who, float *workspace, int
     const int64_t need = tc_floats(d, pl);
     if (need && (!workspace || floats < need))
       return aib_set_errorf("%s: needs a workspace of %lld floats", who, (long long)need), AIB_EINVAL;
-    const int rc = d.hd <= 64 ? launch_tc<64>(d, tree, pl, who, workspace, status, st)
-                              : launch_tc<128>(d, tree, pl, who, workspace, status, st);
+    const bool own = d.hd <= 64 && pl.tpi == 2;  // (Cfg has both sides)
+    const int rc = own          ? launch_tc<64, true>(d, tree, pl, who, workspace, status, st)
+                   : d.hd <= 64 ? launch_tc<64, false>(d, tree, pl, who, workspace, status, st)
+                                : launch_tc<128, false>(d, tree, pl, who, workspace, status, st);
     if (rc != kNoMaps) return rc;
   }
   const int64_t rows = (tree ? d.batch : 1) * d.tokens * d.nh;

@@ -173,6 +173,27 @@ def test_one_key_and_value_for_all_heads_by_an_expanded_tensor():
     R.check(_ops().prompt_attention(q, k, v, _i([0, 90]), 0.1), *R.prompt(q, k, v, _i([0, 90]), 0.1)[:2])
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (3, 1, 48), (8, 2, 128)])
+def test_two_tiles_over_many_keys_with_values_that_are_not_finite(nh, nkv, hd):
+    """One SM to count on, so that every block has two tiles; more key tiles than the ring holds, bad ones among them."""
+    g = _gen(71)
+    lens = [1500, 1, 130, 900]
+    n = sum(lens)
+    q, k, v = _n(g, n, nh, hd, by=1.5), _n(g, n, nkv, hd), _n(g, n, nkv, hd)
+    for i, row in enumerate((130, 700, 1100, 1499, 1631, 2100, n - 1)):
+        v[row, 0, i % hd] = (float("nan"), float("inf"), float("-inf"))[i % 3]
+    cu = _cu(lens)
+    want = R.prompt(q, k, v, cu, 0.1)[:2]
+    for _ in range(3):
+        R.check(_ops().prompt_attention(q, k, v, cu, 0.1, sms=1), *want)
+    t = 200
+    q, k, v = _n(g, 2, t, nh, hd, by=1.5), _n(g, 2, nkv, 1700, hd), _n(g, 2, nkv, 1700, hd)
+    v[0, 0, 1350, 1] = float("nan")  # a column of the mask
+    v[1, 0, 40, 2] = float("inf")
+    mask = torch.rand(2, t, t, device=DEV, generator=g) < 0.2
+    R.check(_ops().tree_attention(q, k, v, _i([1300, 1]), mask, 0.1, sms=1), *R.tree(q, k, v, [1300, 1], mask, 0.1))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
 def test_scales_that_are_not_positive(scale):
     g = _gen(60)
