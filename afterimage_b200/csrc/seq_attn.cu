@@ -650,8 +650,9 @@ __device__ __forceinline__ void join_cluster(const TcParams &p, uint32_t part, i
   const int row = threadIdx.x & (kTile - 1);
   if (row >= field(kCnt0) * p.group) return;
   const int shares = min(p.splits, field(kShares));
-  const int width = HDP / p.splits / 2;  // columns of a thread: 4 (16 shares) to 32 (2)
-  const int c0 = rank * (HDP / p.splits) + static_cast<int>(threadIdx.x >> 7) * width;
+  // columns of a thread: 4 to 32; four columns of a CTA (16 shares, heads of 64) are the first half's alone
+  const int columns = HDP / p.splits, width = max(4, columns / 2);
+  const int c0 = rank * columns + static_cast<int>(threadIdx.x >> 7) * width, c1 = min(c0 + width, (rank + 1) * columns);
   float m = -INFINITY;
 #pragma unroll 4
   for (int s = 0; s < shares; ++s) m = fmaxf(m, ld_cluster(in_cta(part, s) + (HDP * kTile + row) * 4));
@@ -661,7 +662,7 @@ __device__ __forceinline__ void join_cluster(const TcParams &p, uint32_t part, i
                   static_cast<int64_t>(field(kQ0) + field(kT0) + tok) * p.d.out_token_stride +
                   static_cast<int64_t>(kvh * p.group + row - tok * p.group) * p.d.out_head_stride;
 #pragma unroll 1
-  for (int c = c0; c < c0 + width && c < p.d.hd; c += 4) {
+  for (int c = c0; c < c1 && c < p.d.hd; c += 4) {
     float l = 0.f, o[4] = {};
 #pragma unroll 4
     for (int s = 0; s < shares; ++s) {

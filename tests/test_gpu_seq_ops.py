@@ -194,6 +194,22 @@ def test_two_tiles_over_many_keys_with_values_that_are_not_finite(nh, nkv, hd):
     R.check(_ops().tree_attention(q, k, v, _i([1300, 1]), mask, 0.1, sms=1), *R.tree(q, k, v, [1300, 1], mask, 0.1))
 
 
+@pytest.mark.parametrize("sms", [0, 90])
+@pytest.mark.parametrize("nkv", [1, 3, 9, 18])
+@pytest.mark.parametrize("hd", [40, 64, 72, 128])
+def test_every_number_of_shares(hd, nkv, sms):
+    """2, 4, 8 and 16 shares of the key axis in a cluster, others with a second kernel."""
+    g = _gen(73 + hd)
+    mask, _ = _ops().tree_mask([-1, 0, 1, 1, 0], DEV)
+    for rows in (300, 900, 1900, 3000, 5000):
+        q, k, v = _n(g, 1, 5, 4 * nkv, hd, by=1.5), _n(g, 1, nkv, rows, hd), _n(g, 1, nkv, rows, hd)
+        for pos in (rows - 5, rows // 2, 0):
+            R.check(_ops().tree_attention(q, k, v, _i([pos]), mask, hd ** -0.5, sms=sms),
+                    *R.tree(q, k, v, [pos], mask, hd ** -0.5))
+        R.check(_ops().prompt_attention(q[0], k, v, _cu([5]), hd ** -0.5, len_k=_i([rows]), sms=sms),
+                *R.prompt(q[0], k, v, _cu([5]), hd ** -0.5, len_k=_i([rows]))[:2])
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
 def test_scales_that_are_not_positive(scale):
     g = _gen(60)
