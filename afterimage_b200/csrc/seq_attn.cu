@@ -1326,15 +1326,15 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     float4 x[kJoinBatch][2];
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
-      const float4 *r = q + min(s0 + b, last) * (share / 4);  // behind the last share: again the last, times zero
+      const float4 *r = q + min(s0 + b, last) * (share / 4);  // behind the last share: again the last, not added
       x[b][0] = __ldcg(r);
       x[b][1] = __ldcg(r + kTile);
     }
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
-      const int sp = min(s0 + b, last);
-      const float a = s0 + b <= last ? ex2(weight[sp][lane] - ref) : 0.f;
-      l += a * sums[sp][lane];
+      if (s0 + b > last) break;
+      const float a = ex2(weight[s0 + b][lane] - ref);
+      l += a * sums[s0 + b][lane];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         o[4 * i] += a * x[b][i].x;

@@ -210,6 +210,24 @@ def test_every_number_of_shares(hd, nkv, sms):
                 *R.prompt(q[0], k, v, _cu([5]), hd ** -0.5, len_k=_i([rows]))[:2])
 
 
+@pytest.mark.parametrize("sms", [0, 20, 100])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_infinite_values_in_the_last_share(hd, sms):
+    """A value that every row sees is infinite: so is the output, whichever way the shares of the key axis are joined."""
+    g = _gen(72)
+    q, k, v = _n(g, 1, 5, 8, hd), _n(g, 1, 2, 3000, hd), _n(g, 1, 2, 3000, hd)
+    v[0, 0, 2890, 3] = float("inf")
+    v[0, 1, 2700, 1] = float("-inf")
+    v[0, 1, 10, 2] = float("inf")
+    mask, _ = _ops().tree_mask([-1, 0, 1, 1, 0], DEV)
+    want, size = R.tree(q, k, v, [2900], mask, 0.1)
+    assert torch.isinf(want).sum() == 5 * 4 * 3
+    R.check(_ops().tree_attention(q, k, v, _i([2900]), mask, 0.1, sms=sms), want, size)
+    cu = _cu([5])
+    R.check(_ops().prompt_attention(q[0], k, v, cu, 0.1, len_k=_i([2905]), sms=sms),
+            *R.prompt(q[0], k, v, cu, 0.1, len_k=_i([2905]))[:2])
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
 def test_scales_that_are_not_positive(scale):
     g = _gen(60)
