@@ -203,11 +203,12 @@ __global__ void __launch_bounds__(kPlainWarps * 32) attn_plain_kernel(const aib_
 // each (2048 clocks) and 256 exponentials a scheduler at 8 clocks each (2048
 // clocks); the two would have to overlap in full, and tensor memory has no room
 // for a second S beside two O of 128 columns, so that a stream's next scores
-// wait for its product with V (64 columns leave the room). Measured: about 3600 clocks, tensor pipe and
-// exponential unit both busy half of the time. One prompt of 16384 tokens, 40
-// heads of 128 on 8 kv heads, causal: 2.15 ms in a burst (1280 TFLOP/s, 0.77 of
-// the measured cuBLAS burst), 2.65 ms in a loop of seconds (1040, 0.75 of cuBLAS
-// in such a loop), where the power limit holds the clock at 1.67 GHz.
+// wait for its product with V (64 columns leave the room). Measured: about
+// 3600 clocks, tensor pipe and exponential unit both busy half of the time. One
+// prompt of 16384 tokens, 40 heads of 128 on 8 kv heads, causal: 2.15 ms in a
+// burst (1280 TFLOP/s, 0.77 of the measured cuBLAS burst), 2.65 ms in a loop of
+// seconds (1040, 0.75 of cuBLAS in such a loop), where the power limit holds
+// the clock at 1.67 GHz.
 // What was tried and did not pay there: exponentials by a polynomial on the
 // multiply-add pipe for 1/8 or 2/8 of the weights (2.14 -> 2.16 and 2.19 ms); S
 // in halves of 64 keys, the two in turn (2.41 against 2.31 ms then: a product
@@ -1460,7 +1461,8 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int device_sms) {
   // not, one tile a CTA and a share of the key axis. 64 nodes over 32,000 slots: 497 us with two tiles and no shares,
   // 253 us with one tile and none, 86 us with two and nine shares, 63 us with one and six; 317 queries of two prompts
   // over 8000 and 4100 keys, one kv head: 134, 77, 31 and 28 us. Sixteen sequences of 26 nodes fill 128 of 148 SMs
-  // and are not shared out: 36 us, with two, three and four shares each 37, 40 and 43 us.
+  // and are not shared out: 32 us, with two and four shares in clusters 37 and 50 us, and with two, three and four
+  // joined by a second kernel 1, 4 and 7 us more.
   if (pl.items * d.nkv < sms) {
     pl.tpi = 1;
     pl.items = item_bound(d, tree, pl.tt);
