@@ -238,6 +238,11 @@ class KVCache:
         self.lengths[0] = n
 
 
+def _check_one_sequence(who: str, cache: KVCache) -> None:
+    if len(cache.lengths) != 1:
+        raise ValueError("%s: a cache of one sequence, not of %d" % (who, len(cache.lengths)))
+
+
 class _StepState:
     """Static buffers of the graphed single-token step."""
 
@@ -696,7 +701,10 @@ class TPDecoder:
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, cache: KVCache | None = None) -> torch.Tensor:
         """Logits [T, vocab] for the T tokens of `input_ids` (batch 1),
-        appended to `cache` when given."""
+        appended to `cache` (of one sequence; forward_packed takes several)
+        when given."""
+        if cache is not None:
+            _check_one_sequence("forward", cache)
         ids = input_ids.reshape(-1).to(self.device)
         start = cache.length if cache is not None else 0
         T = ids.shape[0]

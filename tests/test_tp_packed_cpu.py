@@ -125,3 +125,24 @@ def test_tree_speculation_refuses():
     for branch in ((), (0,), (cfg.vocab_size + 1,)):
         with pytest.raises(ValueError, match="branch"):
             dec.generate_speculative_tree(ids, 4, dec, branch)
+
+
+def _three(dec, vocab):
+    """A cache of three sequences of different lengths, and a copy of what it holds."""
+    cache = _cache(dec, 40, batch=3)
+    dec.forward_packed([_ids(n, vocab, n) for n in (7, 4, 19)], cache)
+    return cache, [c.clone() for c in cache.k + cache.v]
+
+
+def _unchanged(cache, held, lengths):
+    assert cache.lengths == lengths
+    assert all(torch.equal(a, b) for a, b in zip(cache.k + cache.v, held))
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 5])
+def test_a_forward_of_one_sequence_refuses_a_cache_of_several(tokens):
+    cfg, _, dec = _dec()
+    cache, held = _three(dec, cfg.vocab_size)
+    with pytest.raises(ValueError, match="forward: a cache of one sequence"):
+        dec.forward(_ids(tokens, cfg.vocab_size, 1), cache)
+    _unchanged(cache, held, [7, 4, 19])
