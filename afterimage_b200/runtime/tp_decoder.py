@@ -675,7 +675,9 @@ class TPDecoder:
     def keep_drafted(self, cache: KVCache, path: list) -> None:
         """Commits the drafted tokens `path` (ascending numbers of a tree
         given to forward_tree): their keys and values move to the rows right
-        behind the committed ones, in all layers, and count as committed."""
+        behind the committed ones of `cache` (one sequence), in all layers,
+        and count as committed."""
+        _check_one_sequence("keep_drafted", cache)
         if any(b <= a for a, b in zip(path, path[1:])) or (path and path[0] < 0):
             raise ValueError("keep_drafted: the path's nodes must ascend")
         if path and cache.length + path[-1] >= cache.max_len:

@@ -146,3 +146,12 @@ def test_a_forward_of_one_sequence_refuses_a_cache_of_several(tokens):
     with pytest.raises(ValueError, match="forward: a cache of one sequence"):
         dec.forward(_ids(tokens, cfg.vocab_size, 1), cache)
     _unchanged(cache, held, [7, 4, 19])
+
+
+@pytest.mark.parametrize("path", [[], [0], [0, 1, 2], [0, 2], [3]])
+def test_keeping_a_path_refuses_a_cache_of_several_sequences(path):
+    cfg, _, dec = _dec()
+    cache, held = _three(dec, cfg.vocab_size)
+    with pytest.raises(ValueError, match="keep_drafted: a cache of one sequence"):
+        dec.keep_drafted(cache, path)
+    _unchanged(cache, held, [7, 4, 19])
