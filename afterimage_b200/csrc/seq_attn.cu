@@ -1620,6 +1620,8 @@ static int launch(const aib_attn_desc &d, const char *who, float *workspace, int
     const int64_t need = tc_floats(d, pl);
     if (need && (!workspace || floats < need))
       return aib_set_errorf("%s: needs a workspace of %lld floats", who, (long long)need), AIB_EINVAL;
+    if (need && !aligned16(workspace))  // shares are written and read four floats at a time
+      return aib_set_errorf("%s: the workspace must start on a 16-byte boundary", who), AIB_EINVAL;
     const bool own = d.hd <= 64 && pl.tpi == 2;  // (Cfg has both sides)
     const int rc = own          ? launch_tc<64, true>(d, tree, pl, who, workspace, status, st)
                    : d.hd <= 64 ? launch_tc<64, false>(d, tree, pl, who, workspace, status, st)

@@ -356,8 +356,8 @@ typedef struct aib_attn_desc {
 } aib_attn_desc;
 
 /* Floats of workspace the descriptor's call needs on the current device (0:
- * none). Each call in flight needs its own; nothing in it needs to start at
- * zero. */
+ * none). Each call in flight needs its own, on a 16-byte boundary; nothing in
+ * it needs to start at zero. */
 int64_t aib_attention_workspace_floats(const aib_attn_desc *desc);
 /* Causal attention of packed prompts: sequence b has the query rows
  * cu_q[b] .. cu_q[b + 1] - 1 (m of them) and L keys; its row i sees the keys

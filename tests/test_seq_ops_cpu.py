@@ -208,3 +208,29 @@ def test_cache_c_entries_refuse():
     assert keep(n=257) == _lib.AIB_EINVAL and b"at most 256" in L.aib_last_error()
     assert keep(nkv=0) == _lib.AIB_EINVAL
     assert keep(n=0) == _lib.AIB_OK and keep(count=0) == _lib.AIB_OK
+
+
+@pytest.mark.parametrize("entry,kw", [
+    ("aib_tree_attention_bf16", {}),
+    ("aib_prompt_attention_bf16", dict(mask=None, pos=None, mask_cols=0, cu_k=None, len_k=0x8000)),
+])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_c_entries_refuse_a_workspace_that_is_null_small_or_not_on_16_bytes(entry, kw, hd):
+    """On the host alone: with sms given, the shares join through the workspace (no cluster) on every machine."""
+    L = _lib.load()
+    d = _desc(hd=hd, key_rows=4096, sms=100, **kw)
+    for name in ("q", "k", "v", "out"):
+        setattr(d, name + "_token_stride", 4 * hd)
+        setattr(d, name + "_head_stride", hd)
+    for name in ("k", "v"):
+        setattr(d, name + "_token_stride", hd)
+        setattr(d, name + "_head_stride", 4096 * hd)
+    need = L.aib_attention_workspace_floats(ctypes.byref(d))
+    assert need > 0
+    call = getattr(L, entry)
+    for ptr, floats in ((None, need), (0x10000, need - 1)):
+        assert call(ctypes.byref(d), ptr, floats, None, None) == _lib.AIB_EINVAL
+        assert b"workspace of" in L.aib_last_error()
+    for off in (4, 8, 12):
+        assert call(ctypes.byref(d), 0x10000 + off, need, None, None) == _lib.AIB_EINVAL
+        assert b"16" in L.aib_last_error()
