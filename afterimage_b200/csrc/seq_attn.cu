@@ -1670,6 +1670,10 @@ AIB_API int aib_tree_attention_bf16(const aib_attn_desc *desc, float *workspace,
 
 AIB_API int64_t aib_attention_workspace_floats(const aib_attn_desc *d) {
   if (check_common(d, "attention_workspace_floats") || d->tokens == 0 || d->batch == 0) return 0;
-  const bool tree = d->mask != nullptr;
-  return tensor_cores(*d, tree) ? tc_floats(*d, tc_plan(*d, tree, sm_count())) : 0;
+  const auto floats = [&](bool tree) {
+    return tensor_cores(*d, tree) ? tc_floats(*d, tc_plan(*d, tree, sm_count())) : 0;
+  };
+  // the prompt entry does not look at the mask, nor the tree entry at cu_q: what has both does for either
+  if (!d->mask) return floats(false);
+  return d->cu_q ? std::max(floats(false), floats(true)) : floats(true);
 }

@@ -356,7 +356,7 @@ typedef struct aib_attn_desc {
 } aib_attn_desc;
 
 /* Floats of workspace the descriptor's call needs on the current device (0:
- * none). Each call in flight needs its own, on a 16-byte boundary; nothing in
+ * none); with both cu_q and mask set, what does for either entry. Each call in flight needs its own, on a 16-byte boundary; nothing in
  * it needs to start at zero. */
 int64_t aib_attention_workspace_floats(const aib_attn_desc *desc);
 /* Causal attention of packed prompts: sequence b has the query rows

@@ -234,3 +234,35 @@ def test_attention_c_entries_refuse_a_workspace_that_is_null_small_or_not_on_16_
     for off in (4, 8, 12):
         assert call(ctypes.byref(d), 0x10000 + off, need, None, None) == _lib.AIB_EINVAL
         assert b"16" in L.aib_last_error()
+
+
+@pytest.mark.parametrize("batch,tokens", [(1, 4), (8, 100), (3, 400), (16, 33), (40, 41), (2, 1000)])
+def test_a_descriptor_with_the_fields_of_both_kinds_gets_a_workspace_for_either(batch, tokens):
+    """The prompt entry does not look at the mask, nor the tree entry at cu_q: the size has to do for both. On the host
+    alone: an address off 16 bytes is refused, and only after the size was found to do."""
+    L = _lib.load()
+    hd, rows = 128, 4096
+
+    def desc(**kw):
+        d = _desc(hd=hd, key_rows=rows, sms=100, batch=batch, tokens=tokens, cu_k=None, len_k=0x8000)
+        d.q_batch_stride = d.out_batch_stride = tokens * 4 * hd
+        d.k_batch_stride = d.v_batch_stride = 2 * rows * hd
+        for name in ("q", "out"):
+            setattr(d, name + "_token_stride", 4 * hd)
+            setattr(d, name + "_head_stride", hd)
+        for name in ("k", "v"):
+            setattr(d, name + "_token_stride", hd)
+            setattr(d, name + "_head_stride", rows * hd)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def floats(**kw):
+        return L.aib_attention_workspace_floats(ctypes.byref(desc(**kw)))
+
+    tree, prompt, both = floats(cu_q=None, len_k=None), floats(mask=None, pos=None), floats()
+    assert both == max(tree, prompt)
+    for entry, need in (("aib_tree_attention_bf16", tree), ("aib_prompt_attention_bf16", prompt)):
+        if need:
+            assert getattr(L, entry)(ctypes.byref(desc()), 0x10004, both, None, None) == _lib.AIB_EINVAL
+            assert b"16-byte" in L.aib_last_error()
