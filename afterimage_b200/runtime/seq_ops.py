@@ -113,7 +113,7 @@ def _check_prompt(q, k, v, cu_q, cu_k, len_k, out) -> None:
     _check_device(who, q, k, v, cu_q, cu_k, len_k, out)
     _check_bf16(who, q=q, k=k, v=v, out=out)
     if torch.is_grad_enabled():
-        _check_no_grad(who, q, k, v)
+        _check_no_grad(who, q, k, v, out)
     _need(q.dim() == 3, f"{who}: q must be [tokens, heads, head size]")
     n, nh, hd = q.shape
     _need(cu_q.dim() == 1 and cu_q.shape[0] >= 1, f"{who}: cu_q must be int64 [sequences + 1]")
@@ -184,7 +184,7 @@ def _check_tree(q, k_cache, v_cache, pos, mask, out) -> None:
     _check_device(who, q, k_cache, v_cache, pos, mask, out)
     _check_bf16(who, q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     if torch.is_grad_enabled():
-        _check_no_grad(who, q, k_cache, v_cache)
+        _check_no_grad(who, q, k_cache, v_cache, out)
     _need(q.dim() == 4, f"{who}: q must be [sequences, tokens, heads, head size]")
     b, t, nh, hd = q.shape
     _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.shape[0] == b and k_cache.shape[3] == hd,
@@ -241,7 +241,7 @@ def _check_rope(qkv, nh, nkv, hd, cu, start, inv_freq, k_cache, v_cache, depth, 
     _check_device(who, qkv, cu, start, inv_freq, k_cache, v_cache, depth, q_norm, k_norm, out)
     _check_bf16(who, qkv=qkv, k_cache=k_cache, v_cache=v_cache, q_norm=q_norm, k_norm=k_norm, out=out)
     if torch.is_grad_enabled():
-        _check_no_grad(who, qkv, q_norm, k_norm)
+        _check_no_grad(who, qkv, inv_freq, k_cache, v_cache, q_norm, k_norm, out)
     _need(nh > 0 and nkv > 0 and hd >= 2 and hd % 2 == 0 and hd <= 1024, f"{who}: bad heads or head size")
     _need(qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * hd, f"{who}: qkv must be [N, {(nh + 2 * nkv) * hd}]")
     n = qkv.shape[0]
@@ -299,7 +299,7 @@ def rope_cache_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, cu: torch.T
                   and q_norm.dim() == 1 and k_norm.dim() == 1 and q_norm.shape[0] == hd and k_norm.shape[0] == hd
                   and q_norm.stride(0) == 1 and k_norm.stride(0) == 1 and q_norm.get_device() == dev
                   and k_norm.get_device() == dev)
-             and _no_grad(qkv, q_norm, k_norm))
+             and _no_grad(qkv, inv_freq, k_cache, v_cache, q_norm, k_norm))
     if not usual:
         _check_rope(qkv, nh, nkv, hd, cu, start, inv_freq, k_cache, v_cache, depth, q_norm, k_norm, out)
         _check_cuda("rope_cache_packed", qkv)
@@ -326,6 +326,7 @@ def rope_cache_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, cu: torch.T
 
 
 _shape_of, _dtype_of = torch.Tensor.shape.__get__, torch.Tensor.dtype.__get__
+_needs_grad = torch.Tensor.requires_grad.__get__
 
 
 def _all_are(values, value, n: int) -> bool:
@@ -336,6 +337,8 @@ def _check_keep(caches, pos, keep, ptrs) -> None:
     who = "keep_cache_rows"
     first = caches[0]
     _check_device(who, first, pos, keep)
+    if torch.is_grad_enabled():
+        _check_no_grad(who, *caches)
     _need(first.dim() == 4, f"{who}: caches must be [B, kv heads, max_len, head size]")
     for t in caches:
         _need(t.dtype == _BF16 and t.shape == first.shape and t.stride() == first.stride() and t.device == first.device,
@@ -371,7 +374,7 @@ def keep_cache_rows(caches: list, pos: torch.Tensor, keep: torch.Tensor) -> None
              and strides[3] == 1 and min(strides) > 0 and pos.dtype is _I64 and keep.dtype is _I64
              and pos.get_device() == dev and keep.get_device() == dev and pos.shape == shape[:1] and keep.dim() == 2
              and keep.shape[0] == shape[0] and keep.shape[1] <= MAX_KEEP and pos.is_contiguous()
-             and keep.is_contiguous())
+             and keep.is_contiguous() and not (torch.is_grad_enabled() and any(map(_needs_grad, caches))))
     if not usual:
         _check_keep(caches, pos, keep, ptrs)
         _check_cuda("keep_cache_rows", first)

@@ -266,3 +266,25 @@ def test_a_descriptor_with_the_fields_of_both_kinds_gets_a_workspace_for_either(
         if need:
             assert getattr(L, entry)(ctypes.byref(desc()), 0x10004, both, None, None) == _lib.AIB_EINVAL
             assert b"16-byte" in L.aib_last_error()
+
+
+def _grad(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype, requires_grad=True)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: _rope(k_cache=_grad(2, 2, 8, 16)),
+    lambda: _rope(v_cache=_grad(2, 2, 8, 16)),
+    lambda: _rope(inv_freq=_grad(8, dtype=torch.float32)),
+    lambda: _rope(out=_grad(5, 4, 16)),
+    lambda: _rope(q_norm=_grad(16), k_norm=torch.ones(16, dtype=BF)),
+    lambda: S.keep_cache_rows([CACHE, _grad(2, 2, 8, 16)], _i(0, 1), torch.zeros(2, 3, dtype=torch.int64)),
+    lambda: S.keep_cache_rows([_grad(2, 2, 8, 16)], _i(0, 1), torch.zeros(2, 3, dtype=torch.int64)),
+    lambda: _prompt(out=_grad(6, 4, 16)),
+    lambda: _tree(out=_grad(2, 3, 4, 16)),
+], ids=["rope k", "rope v", "rope inv_freq", "rope out", "rope norms", "keep second", "keep first", "prompt out", "tree out"])
+def test_tensors_that_need_a_gradient_are_refused(call):
+    with pytest.raises(ValueError, match="backward"):
+        call()
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # nothing but the device is wrong then
+        call()
