@@ -220,7 +220,8 @@ def _rotate_half(x: torch.Tensor) -> torch.Tensor:
 
 class KVCache:
     """Static per-rank cache: [layers][2] tensors of [batch, kv_heads_local, max_len, head_dim]. `lengths` counts the
-    tokens of each sequence; `length` is the first one's (the only one's, where a forward takes a single sequence)."""
+    tokens of each sequence; `length` is the first one's (the only one's, where a forward takes a single sequence).
+    `drafted` counts the rows behind `length` that hold a tree's nodes (TPDecoder.forward_tree)."""
 
     def __init__(self, n_layers, kv_heads, head_dim, max_len, device, dtype=torch.bfloat16, batch=1):
         shape = (batch, kv_heads, max_len, head_dim)
@@ -228,6 +229,15 @@ class KVCache:
         self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(n_layers)]
         self.max_len = max_len
         self.lengths = [0] * batch
+        self._drafted = (0, 0)  # the length that the nodes stand behind, and how many they are
+
+    @property
+    def drafted(self) -> int:
+        return self._drafted[1] if self._drafted[0] == self.length else 0
+
+    @drafted.setter
+    def drafted(self, n: int) -> None:
+        self._drafted = (self.length, n)
 
     @property
     def length(self) -> int:
@@ -612,6 +622,7 @@ class TPDecoder:
         for m in lens:
             cu.append(cu[-1] + m)
         ids = torch.cat([p.reshape(-1).to(self.device) for p in prompts])
+        cache.drafted = 0  # its rows are written over
         self.begin_forward()
         x = self.embed(ids)
         if self.fused:
@@ -654,6 +665,7 @@ class TPDecoder:
             raise ValueError("forward_tree: %d tokens for a cache of %d" % (pos + C, cache.max_len))
         mask, depth = mask.to(self.device), depth.to(self.device)
         first = pos + C - T
+        cache.drafted = min(cache.drafted, C - T)  # rows from there on are written over
         self.begin_forward()
         x = self.embed(ids)
         if self.fused:
@@ -670,6 +682,7 @@ class TPDecoder:
 
         # rotary places count from the first row of this call
         x = self._layers_rows(x, cache, [0, T], [first], depth - (C - T), attend, attend_plain)
+        cache.drafted = C
         return self._all_gather_last(self.head_logits(x))
 
     def keep_drafted(self, cache: KVCache, path: list) -> None:
@@ -682,6 +695,9 @@ class TPDecoder:
             raise ValueError("keep_drafted: the path's nodes must ascend")
         if path and cache.length + path[-1] >= cache.max_len:
             raise ValueError("keep_drafted: node %d lies behind the cache" % path[-1])
+        if path and path[-1] >= cache.drafted:
+            raise ValueError("keep_drafted: node %d was never run (forward_tree left %d nodes behind the committed "
+                             "tokens)" % (path[-1], cache.drafted))
         if list(path) != list(range(len(path))):
             if self.fused:
                 from . import seq_ops
@@ -692,6 +708,8 @@ class TPDecoder:
                 src = torch.tensor(path, device=self.device) + cache.length
                 for c in cache.k + cache.v:
                     c[:, :, cache.length:cache.length + len(path)] = c[:, :, src]
+        if path:
+            cache.drafted = 0  # the tree's numbers have gone with the rows that were kept
         cache.length += len(path)
 
     def embed(self, ids: torch.Tensor) -> torch.Tensor:
@@ -707,6 +725,7 @@ class TPDecoder:
         when given."""
         if cache is not None:
             _check_one_sequence("forward", cache)
+            cache.drafted = 0  # its rows are written over
         ids = input_ids.reshape(-1).to(self.device)
         start = cache.length if cache is not None else 0
         T = ids.shape[0]

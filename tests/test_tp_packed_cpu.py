@@ -155,3 +155,43 @@ def test_keeping_a_path_refuses_a_cache_of_several_sequences(path):
     with pytest.raises(ValueError, match="keep_drafted: a cache of one sequence"):
         dec.keep_drafted(cache, path)
     _unchanged(cache, held, [7, 4, 19])
+
+
+def test_nodes_that_were_never_run_are_not_kept():
+    from afterimage_b200.runtime.seq_ops import tree_mask
+    cfg, _, dec = _dec()
+    cache = _cache(dec, 40)
+    dec.forward_packed([_ids(7, cfg.vocab_size, 0)], cache)
+    mask, depth = tree_mask([-1, 0, 0, 1, 2])
+
+    def refused(*paths):
+        held, n = [c.clone() for c in cache.k + cache.v], cache.length
+        for path in paths:
+            with pytest.raises(ValueError, match="never run"):
+                dec.keep_drafted(cache, path)
+        _unchanged(cache, held, [n])
+
+    refused([0], [0, 1, 2, 3, 4])           # no tree at all
+    dec.forward_tree(_ids(3, cfg.vocab_size, 1), mask[:3, :3], depth[:3], cache)
+    refused([3], [0, 1, 3])                 # a tree of three
+    dec.forward_tree(_ids(2, cfg.vocab_size, 2), mask[3:], depth[3:], cache)
+    refused([5], [0, 2, 5])                 # the same, with two more
+    dec.keep_drafted(cache, [])             # keeps nothing, and the tree stands
+    dec.keep_drafted(cache, [0, 2, 4])
+    assert cache.length == 10
+    refused([0], [1])                       # the tree is gone with its numbers
+    cache.length = 7
+    refused([0], [1])
+    cache.length = 10
+    for write in (lambda: dec.forward(_ids(1, cfg.vocab_size, 3), cache),
+                  lambda: dec.forward(_ids(2, cfg.vocab_size, 3), cache),
+                  lambda: dec.forward_packed([_ids(2, cfg.vocab_size, 3)], cache)):
+        dec.forward_tree(_ids(5, cfg.vocab_size, 4), mask, depth, cache)
+        n = cache.length
+        write()
+        refused([0], [1])                   # its rows are written over
+        cache.length = n
+        refused([0], [1])                   # and stay so when the tokens are cut again
+    dec.forward_tree(_ids(2, cfg.vocab_size, 5), mask[:2, :2], depth[:2], cache)
+    cache.length -= 1
+    refused([0], [1])                       # its numbers count from another row now
