@@ -34,7 +34,8 @@ MAX_KEEP = 256
 _DESC = struct.Struct("@4P15q3if5P5q")
 assert _DESC.size == ctypes.sizeof(_lib.AttnDesc)
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# (absent from a torch without CUDA, which has no tensors that get as far)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _need(ok: bool, text: str) -> None:

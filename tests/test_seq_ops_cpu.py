@@ -288,3 +288,22 @@ def test_tensors_that_need_a_gradient_are_refused(call):
         call()
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # nothing but the device is wrong then
         call()
+
+
+def test_a_torch_without_cuda_imports_the_operators(tmp_path):
+    """CPU ranks use tree_mask; the operators themselves still ask for CUDA tensors."""
+    import pathlib
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n    delattr(torch._C, n)\n"
+            "from afterimage_b200.runtime import seq_ops as S\n"
+            "assert S.tree_mask([-1, 0])[1].tolist() == [0, 1]\n"
+            "c = torch.zeros(1, 1, 4, 8, dtype=torch.bfloat16)\n"
+            "i = torch.zeros(1, dtype=torch.int64)\n"
+            "try:\n    S.keep_cache_rows([c], i, i[None])\n"
+            "except ValueError as e:\n    assert 'CUDA' in str(e), e\n"
+            "else:\n    raise AssertionError('not refused')\n")
+    root = pathlib.Path(_lib.__file__).resolve().parent.parent
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
