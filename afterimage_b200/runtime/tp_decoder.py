@@ -607,7 +607,8 @@ class TPDecoder:
         product over all tokens. Returns the logits after each sequence's
         last token, [len(prompts), vocab]. The fused mode runs the packed
         kernels of seq_ops; results agree with forward() up to BF16
-        rounding."""
+        rounding. Waits for the pass, and raises where its kernels set a
+        status bit."""
         if len(prompts) != len(cache.lengths):
             raise ValueError("forward_packed: %d prompts for a cache of %d sequences" % (len(prompts),
                                                                                       len(cache.lengths)))
@@ -642,9 +643,11 @@ class TPDecoder:
             return torch.cat(out)
 
         x = self._layers_rows(x, cache, cu, start, None, attend, attend_plain)
-        cache.lengths = ends
         last = torch.tensor([c - 1 for c in cu[1:]], device=x.device)
-        return self._all_gather_last(self.head_logits(x[last]))
+        logits = self._all_gather_last(self.head_logits(x[last]))
+        _device.check_status(self.device)  # a wait that gave up, or a corrupt stream, commits nothing
+        cache.lengths = ends
+        return logits
 
     @torch.no_grad()
     def forward_tree(self, ids: torch.Tensor, mask: torch.Tensor, depth: torch.Tensor, cache: KVCache) -> torch.Tensor:
@@ -655,7 +658,8 @@ class TPDecoder:
         (itself among them); depth int64 [T]: its distance from the first
         place behind the committed tokens (seq_ops.tree_mask makes both).
         Their keys and values stay in the rows behind cache.length, which
-        does not change: keep_drafted commits a path of them."""
+        does not change: keep_drafted commits a path of them. Waits for the
+        pass, and raises where its kernels set a status bit."""
         ids = ids.reshape(-1).to(self.device)
         T, C = mask.shape
         pos = cache.length
@@ -682,8 +686,10 @@ class TPDecoder:
 
         # rotary places count from the first row of this call
         x = self._layers_rows(x, cache, [0, T], [first], depth - (C - T), attend, attend_plain)
+        logits = self._all_gather_last(self.head_logits(x))
+        _device.check_status(self.device)
         cache.drafted = C
-        return self._all_gather_last(self.head_logits(x))
+        return logits
 
     def keep_drafted(self, cache: KVCache, path: list) -> None:
         """Commits the drafted tokens `path` (ascending numbers of a tree

@@ -90,3 +90,29 @@ def test_tree_speculation_is_greedy_decoding(stored, resident, branch):
         _check_greedy(got, want, margins, 9)
         assert stats["accepted_from_draft"] >= least, stats
     dec.close()
+
+
+@pytest.mark.parametrize("resident", ["decoded", "compressed"])
+def test_a_status_bit_raises_and_commits_nothing(stored, resident):
+    from afterimage_b200 import _lib
+    from afterimage_b200.runtime import _device
+    from afterimage_b200.runtime.seq_ops import tree_mask
+    from afterimage_b200.runtime.tp_decoder import load_tp_decoder
+    cfg, model, store = stored
+    dec = load_tp_decoder(store, cfg, 1, 0, None, "cuda", resident=resident)
+    cache = _cache(dec, 40)
+    ids = _ids(7, cfg.vocab_size, 8)
+    mask, depth = tree_mask([-1, 0, 0], "cuda")
+    word = _device.status_word(torch.device("cuda", torch.cuda.current_device()))
+    word.fill_(_lib.STATUS_WAIT_TIMEOUT)  # as a wait that gives up leaves it
+    with pytest.raises(RuntimeError, match="timed out"):
+        dec.forward_packed([ids], cache)
+    assert cache.lengths == [0]
+    dec.forward_packed([ids], cache)  # the word was cleared
+    word.fill_(_lib.STATUS_WAIT_TIMEOUT)
+    with pytest.raises(RuntimeError, match="timed out"):
+        dec.forward_tree(ids[:3], mask, depth, cache)
+    assert cache.lengths == [7] and cache.drafted == 0
+    check_logits(dec.forward_tree(ids[:3], mask, depth, cache)[0], _ref(model, torch.cat((ids, ids[:1])))[-1],
+                 atol=FUSED_STEP_ATOL)
+    dec.close()

@@ -195,3 +195,26 @@ def test_nodes_that_were_never_run_are_not_kept():
     dec.forward_tree(_ids(2, cfg.vocab_size, 5), mask[:2, :2], depth[:2], cache)
     cache.length -= 1
     refused([0], [1])                       # its numbers count from another row now
+
+
+@pytest.mark.parametrize("fails", ["forward_packed", "forward_tree"])
+def test_a_pass_whose_kernels_gave_up_raises_and_commits_nothing(monkeypatch, fails):
+    """A bounded wait that gives up leaves rows unwritten and sets the status word (stood in for here)."""
+    from afterimage_b200.runtime import tp_decoder
+    from afterimage_b200.runtime.seq_ops import tree_mask
+    cfg, _, dec = _dec()
+    cache = _cache(dec, 40)
+    dec.forward_packed([_ids(7, cfg.vocab_size, 0)], cache)
+    mask, depth = tree_mask([-1, 0, 0])
+
+    def gave_up(dev):
+        raise RuntimeError("a bounded shared-memory copy wait timed out")
+
+    with monkeypatch.context() as m:
+        m.setattr(tp_decoder._device, "check_status", gave_up)
+        with pytest.raises(RuntimeError, match="timed out"):
+            if fails == "forward_packed":
+                dec.forward_packed([_ids(2, cfg.vocab_size, 1)], cache)
+            else:
+                dec.forward_tree(_ids(3, cfg.vocab_size, 1), mask, depth, cache)
+    assert cache.lengths == [7] and cache.drafted == 0
