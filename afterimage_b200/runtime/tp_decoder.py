@@ -297,7 +297,7 @@ class TPDecoder:
         self.timeline = None  # a list to record (kind, layer, start event, end event) into
         self._graph_state = None
         self.allreducer = None  # one-shot NVLink all-reduce (use_oneshot_allreduce); else NCCL
-        self.free_sms = 0       # SMs that the layer math may count on (0: all); fewer beside an overlapped decode
+        self.attention_sms = 0  # seq_ops' `sms`: 0, but all of them by number beside an overlapped decode
         rp = getattr(hf_cfg, "rope_parameters", None) or {}
         theta = rp.get("rope_theta", getattr(hf_cfg, "rope_theta", 10000.0))
         self.inv_freq = 1.0 / (theta ** (torch.arange(0, self.hd, 2, dtype=torch.int64).to(
@@ -633,7 +633,7 @@ class TPDecoder:
 
         def attend(i, q):
             return seq_ops.prompt_attention(q, cache.k[i], cache.v[i], d_cu, self.hd ** -0.5, len_k=len_k,
-                                            sms=self.free_sms)
+                                            sms=self.attention_sms)
 
         def attend_plain(i, q):
             out = []
@@ -678,7 +678,7 @@ class TPDecoder:
 
         def attend(i, q):
             return seq_ops.tree_attention(q[None], cache.k[i], cache.v[i], d_pos, mask, self.hd ** -0.5,
-                                          sms=self.free_sms)[0]
+                                          sms=self.attention_sms)[0]
 
         def attend_plain(i, q):
             seen = torch.cat((torch.ones(T, pos, dtype=torch.bool, device=q.device), mask), 1)
@@ -1208,8 +1208,13 @@ class CompressedTPDecoder(TPDecoder):
         if decode_sms is None:
             decode_sms = round(0.78 * torch.cuda.get_device_properties(self.dev).multi_processor_count)
         self.decode_sms = int(decode_sms) if self.overlap else 0
-        if self.decode_sms > 0:
-            self.free_sms = max(1, torch.cuda.get_device_properties(self.dev).multi_processor_count - self.decode_sms)
+        # Beside that decode the attention is cut for every SM, but without clusters, which wait for several free SMs of
+        # one GPC. Microseconds a layer of the 14B shape, decode on 115 SMs, cut for 33 (what it leaves) / 111 / all 148
+        # / 148 with clusters: a token over 1000 slots 429 / 428 / 428 / 478, 26 nodes over 1000 513 / 513 / 516 / 516
+        # and over 20,000 569 / 528 / 526 / 526, 64 nodes over 32,000 597 / 538 / 523 / 524, 256 queries over 8000 642
+        # / 597 / 600 / 600. With the decode on all SMs the same order, but clusters cost nothing.
+        if self.overlap:
+            self.attention_sms = torch.cuda.get_device_properties(self.dev).multi_processor_count
         self._ahead: dict = {}
         # decoded weights land in preallocated output sets (two when the decode of layer
         # i+1 overlaps layer i's projections), so descriptors are built once per

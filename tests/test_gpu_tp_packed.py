@@ -116,3 +116,27 @@ def test_a_status_bit_raises_and_commits_nothing(stored, resident):
     check_logits(dec.forward_tree(ids[:3], mask, depth, cache)[0], _ref(model, torch.cat((ids, ids[:1])))[-1],
                  atol=FUSED_STEP_ATOL)
     dec.close()
+
+
+@pytest.mark.parametrize("kw", [{}, {"decode_sms": 0}, {"decode_sms": 20}, {"decode_sms": 148}, {"decode_sms": 4096}],
+                         ids=str)
+def test_attention_beside_an_overlapped_decode_is_cut_for_every_sm(stored, kw):
+    """Not for the SMs that the decode leaves: a long axis on those alone took longer than waiting for the others."""
+    import ctypes
+
+    from afterimage_b200 import _lib
+    from afterimage_b200.runtime.tp_decoder import load_tp_decoder
+    cfg, _, store = stored
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    dec = load_tp_decoder(store, cfg, 1, 0, None, "cuda", resident="compressed", overlap=True, **kw)
+    assert dec.attention_sms == sms
+    dec.close()
+    # one kv head over 32768 rows: a share for (nearly) every SM
+    d = _lib.AttnDesc(q=0x1000, k=0x2000, v=0x3000, out=0x4000, q_token_stride=512, q_head_stride=128,
+                      out_token_stride=512, out_head_stride=128, k_token_stride=128, v_token_stride=128, tokens=1,
+                      batch=1, key_rows=32768, nh=4, nkv=1, hd=128, scale=1.0, pos=0x6000, mask=0x7000, mask_cols=1,
+                      sms=dec.attention_sms)
+    assert _lib.load().aib_attention_workspace_floats(ctypes.byref(d)) == 64 * 128 * 130
+    dec = load_tp_decoder(store, cfg, 1, 0, None, "cuda", resident="compressed")
+    assert dec.attention_sms == 0  # nothing beside it: all SMs, and clusters
+    dec.close()
