@@ -218,3 +218,19 @@ def test_a_pass_whose_kernels_gave_up_raises_and_commits_nothing(monkeypatch, fa
             else:
                 dec.forward_tree(_ids(3, cfg.vocab_size, 1), mask, depth, cache)
     assert cache.lengths == [7] and cache.drafted == 0
+
+
+@pytest.mark.parametrize("branch", [(2, 2, 1), (2, 2, 2, 2), (3,)])
+def test_tokens_behind_moved_rows_are_greedy_too(branch):
+    """24 tokens, each judged on its own prefix; the draft's second choice is the target's first, so that every sweep
+    goes on from rows that keep_drafted moved together, in both caches."""
+    from greedy_teacher import check_greedy_tokens, check_paths, record_kept, swap_best_two
+    cfg, m, dec = _dec()
+    draft = swap_best_two(_dec()[2])
+    paths, drafts = record_kept(dec), record_kept(draft)
+    got = dec.generate_speculative_tree(_ids(9, cfg.vocab_size, 6), 24, draft, branch)
+    assert got.shape == (1, 33)
+    check_greedy_tokens(m, got, 9, 2e-2)  # (the tolerance of the packed passes above)
+    check_paths(paths, 24)
+    if len(branch) > 1:
+        assert any(p and p != list(range(len(p))) for p in drafts[:-1]), drafts
