@@ -10,7 +10,9 @@
 // A prompt's row i sees the keys j <= L - m + i. A tree's row i sees every
 // cache slot before pos, and slot pos + j where mask[i, j]. A row that sees
 // nothing is zero. What a row does not see cannot reach it: masked scores are
-// replaced, not added to, and a masked v_j is never multiplied.
+// replaced, not added to; the plain kernel never multiplies a masked v_j, and
+// the tensor-core kernel, whose masked weights are zeros that are multiplied,
+// first takes out of V what is not finite (warps 10-11).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -250,7 +252,6 @@ struct TcParams {
   int tpi;             // tiles an item may hold: 2 or 1
   int splits;          // shares of the key axis
   int cluster;         // the shares are one cluster's CTAs and join through its shared memory, without a second kernel
-  int items;           // upper bound of the items
   float scale_log2;
   int vec_out;         // output rows allow 16-byte stores
   float *workspace;    // shares: O, maximum and sum of their rows
@@ -1581,7 +1582,6 @@ static int launch_tc(const aib_attn_desc &d, bool tree, const TcPlan &pl, const 
   p.tpi = pl.tpi;
   p.splits = pl.splits;
   p.cluster = pl.cluster;
-  p.items = static_cast<int>(pl.items);
   p.scale_log2 = d.scale * 1.4426950408889634f;
   p.vec_out = aligned16(d.out) && d.out_token_stride % 8 == 0 && d.out_head_stride % 8 == 0 &&
               d.out_batch_stride % 8 == 0;
