@@ -327,7 +327,6 @@ def rope_cache_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, cu: torch.T
 
 
 _shape_of, _dtype_of = torch.Tensor.shape.__get__, torch.Tensor.dtype.__get__
-_needs_grad = torch.Tensor.requires_grad.__get__
 
 
 def _all_are(values, value, n: int) -> bool:
@@ -375,7 +374,7 @@ def keep_cache_rows(caches: list, pos: torch.Tensor, keep: torch.Tensor) -> None
              and strides[3] == 1 and min(strides) > 0 and pos.dtype is _I64 and keep.dtype is _I64
              and pos.get_device() == dev and keep.get_device() == dev and pos.shape == shape[:1] and keep.dim() == 2
              and keep.shape[0] == shape[0] and keep.shape[1] <= MAX_KEEP and pos.is_contiguous()
-             and keep.is_contiguous() and not (torch.is_grad_enabled() and any(map(_needs_grad, caches))))
+             and keep.is_contiguous() and not (torch.is_grad_enabled() and torch._C._any_requires_grad(*caches)))
     if not usual:
         _check_keep(caches, pos, keep, ptrs)
         _check_cuda("keep_cache_rows", first)
