@@ -639,6 +639,7 @@ __device__ __forceinline__ void add_not_finite(const TcParams &p, const Seq &s, 
         if (not_finite_bf16(x)) o += b2f(x);
       }
     }
+    __syncwarp();  // the lanes went their own ways, and tensor memory is written by a converged warp
     tmem_st1(to + c, o);
   }
   tmem_wait_st();
@@ -1199,6 +1200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (; c < c_end; c += 16) {
         float o[16];
+        __syncwarp();  // lanes without a row left the last round early
         if (mine > 0) {
           tmem_ld16(to + c, reinterpret_cast<uint32_t *>(o));
           tmem_wait_ld();
