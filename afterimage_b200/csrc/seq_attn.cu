@@ -89,7 +89,11 @@ __device__ __forceinline__ bool sees(const aib_attn_desc &p, const Seq &s, int64
 // lane takes one key's score, then the warp adds the seen keys' values, a
 // lane per value column). It takes every head size up to 256 and every
 // stride; scores, sums and the running output are fp32, the result is
-// rounded once.
+// rounded once. It is there to be right, not fast (a warp reads every key for
+// one row): 1024 tokens of 16 heads of 256 on 8 take 8.3 ms, 26 nodes over
+// 4000 slots 3.2 ms, where the same heads of 128 take 16 us each on the tensor
+// cores; a second O of 256 columns beside the scores would need another layout
+// of tensor memory, and no model shape of this package has such heads.
 // ---------------------------------------------------------------------------
 constexpr int kPlainMaxHd = 256;
 constexpr int kPlainWarps = 4;
@@ -1470,7 +1474,9 @@ static TcPlan tc_plan(const aib_attn_desc &d, bool tree, int device_sms) {
     pl.tpi = 1;
     pl.items = item_bound(d, tree, pl.tt);
     const int64_t units = std::max<int64_t>(1, pl.items * d.nkv);
-    // shares of at least two key tiles (one for each stream), at most one CTA per SM
+    // shares of at least two key tiles (one for each stream), at most one CTA per SM. The lengths are on the device, so
+    // the tiles are those of the whole cache: one token over 1000 slots takes 9.5 us in a cache of 1152 rows, 9.6 in
+    // one of 8192 and 12.2 in one of 32,768; 26 nodes 15.0, 15.5 and 15.5.
     const int64_t tiles = (d.key_rows + kTile - 1) / kTile;
     const int64_t cap = std::max<int64_t>(1, sms / units);
     pl.splits = static_cast<int>(std::min<int64_t>(std::min<int64_t>(cap, (tiles + 1) / 2), kMaxSplits));

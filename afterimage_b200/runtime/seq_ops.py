@@ -144,8 +144,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     row i of m sees the keys j <= L - m + i. Rows that see nothing are zero;
     rows of q in no sequence are not computed and their rows of `out` not
     written. Returns out [N, nh, hd] (new unless given; it may be q). `sms`:
-    how many SMs the call may count on while kernels of other streams hold
-    the rest (0: all of them)."""
+    how many SMs the work is cut for while kernels of other streams hold
+    some, without clusters, which wait for several free SMs at once (0: all
+    of them, with clusters where they pay)."""
     shape, kshape = q.shape, k.shape
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     dev = q.get_device()

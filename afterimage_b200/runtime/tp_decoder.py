@@ -604,8 +604,9 @@ class TPDecoder:
         """One pass over several token sequences of different lengths
         (1-D int64 tensors), sequence b appended to entry b of `cache`
         (KVCache(batch=len(prompts))): no padding, every projection one
-        product over all tokens. Returns the logits after each sequence's
-        last token, [len(prompts), vocab]. The fused mode runs the packed
+        product over all tokens. Each sequence needs a token; one that has
+        ended leaves by way of a cache without it. Returns the logits after
+        each sequence's last token, [len(prompts), vocab]. The fused mode runs the packed
         kernels of seq_ops; results agree with forward() up to BF16
         rounding. Waits for the pass, and raises where its kernels set a
         status bit."""

@@ -350,9 +350,9 @@ typedef struct aib_attn_desc {
   const uint8_t *mask;  /* tree: [batch, tokens, mask_cols], nonzero where the query sees the drafted column */
   int64_t mask_batch_stride, mask_row_stride, mask_col_stride;
   int64_t mask_cols;    /* tree: drafted tokens in the cache, at slots pos .. pos + mask_cols - 1 */
-  int64_t sms;          /* SMs that the call may count on beside kernels of other streams (0: all). Where it is given
-                           the work is cut for that many and runs on whatever is free, without clusters, which
-                           would wait for several free SMs of one GPC */
+  int64_t sms;          /* SMs that the work is cut for beside kernels of other streams (0: all). Where it is given the
+                           call runs on whatever is free, without clusters, which would wait for several free SMs of
+                           one GPC; the device's own number is a good choice */
 } aib_attn_desc;
 
 /* Floats of workspace the descriptor's call needs on the current device (0:
